@@ -65,9 +65,11 @@ int mt_mem_info(size_t* free_bytes, size_t* total_bytes);
  * out-of-range index record a code here instead of trapping (the largest code
  * seen is kept). Reads it back (synchronising `stream`) and clears it.
  * 0 = nothing recorded; 1 = embedding index out of range (row skipped);
- * 2 = cross-entropy label out of range (row ignored); an expired bounded wait:
+ * 2 = cross-entropy label out of range (row ignored); 3 = paged cache: no page left, or
+ * a page or slot outside the pool (what it concerned is left out); an expired bounded wait:
  * 100 = tensor-core GEMM, 101 = attention forward, 102 = attention backward,
- * 103 = staged cross entropy, 104 = staged LayerNorm / RMSNorm backward. */
+ * 103 = staged cross entropy, 104 = staged LayerNorm / RMSNorm backward,
+ * 105 = attention over pages. */
 int mt_device_flag_read(int* flag, void* stream);
 
 /* Per-kernel-class timing with CUDA events on the launching stream.
@@ -374,6 +376,52 @@ int mt_kv_append(const void* k_new, const void* v_new, void* k_cache, void* v_ca
                  mt_strides3 sk, mt_strides3 sv, mt_strides3 scache,
                  int64_t batch, int64_t heads, int64_t n_new, int64_t pos0, int64_t max_len,
                  int64_t head_dim, int dtype, void* stream);
+
+/* ---- the paged key/value cache ---------------------------------------------
+ * Requests of different lengths that come and go (no counterpart in the reference, whose Cache,
+ * gpt2_trainer/gpt2.py:29-86, holds one length for a whole batch). A layer's keys and values live in
+ * two pools of n_pages pages of page_size rows, addressed with strides {page, head, row} (the
+ * head_dim stride is 1). Row j of request r is row j % page_size of page tables[r, j / page_size]
+ * (tables int32 [requests, width]). The new tokens of a step are packed: request r has rows
+ * [starts[r], starts[r+1]). Everything a step needs of the lengths is computed on the device, so
+ * nothing here waits for the host and a step can be captured.
+ *
+ * mt_paged_tables: request r holds held[r] rows and gets fresh[r] new ones (negative counts are 0).
+ * Pages ceil(held/page_size) .. ceil((held+fresh)/page_size)-1 of every request, requests in order,
+ * are taken from the end of the list free_pages[0, n_free[0]) (list_len entries of room) and written
+ * to the tables; no other entry changes. Out: starts [requests+1], kv_len = held + fresh, n_free_out
+ * (a buffer of its own, as kv_len is, so the same call may be made again), and for each of `rows`
+ * token rows its position in its request and its slot = page * page_size + row; rows behind the last
+ * token get position 0 and slot -1. A page that is not there (list empty, table too narrow) sets the
+ * device status word; its entry, where the table has one, and its tokens' slots are -1. At most 8192
+ * requests.
+ * mt_paged_release: the pages of the requests with done[r] != 0 go back to the end of the list in the
+ * order of requests and pages, their entries become -1 and kv_len[r] 0. A page may be in one table
+ * only. */
+int mt_paged_tables(const int32_t* held, const int32_t* fresh, int32_t* tables, const int32_t* free_pages,
+                    const int32_t* n_free, int32_t* starts, int32_t* kv_len, int32_t* position, int32_t* slot,
+                    int32_t* n_free_out, int64_t requests, int64_t width, int64_t page_size, int64_t list_len,
+                    int64_t rows, void* stream);
+int mt_paged_release(const int32_t* done, int32_t* tables, int32_t* kv_len, int32_t* free_pages, int32_t* n_free,
+                     int64_t requests, int64_t width, int64_t page_size, int64_t list_len, void* stream);
+/* Row i of k_new / v_new (strides {unused, head, row}) goes to slot[i] of the pools, all kv_heads heads;
+ * a negative slot is skipped, one beyond the pool too (and sets the status word). The slots of one call
+ * are distinct. */
+int mt_paged_append(const void* k_new, const void* v_new, void* k_pages, void* v_pages, mt_strides3 sk,
+                    mt_strides3 sv, mt_strides3 spages, const int32_t* slot, int64_t rows, int64_t kv_heads,
+                    int64_t head_dim, int64_t page_size, int64_t n_pages, int dtype, void* stream);
+/* Attention of every request's new rows over its pages: kv_len[r] counts the keys of request r, its new
+ * ones (already appended) among them; the last new row sees all of them, the row before it one less, and
+ * so on (softmax(scale q.k) v over the visible keys; query head h reads key/value head
+ * h / (heads / kv_heads)). q and o are [rows, heads, head_dim] with strides {unused, head, row}; rows that
+ * no request has are not written. A row that sees no key, or only scores of -inf, is 0; what a row does not see does not
+ * reach it, not even as NaN. Keys on a page outside the pool are left out (status word). max_new: the most
+ * new rows a request is expected to have, which only picks the kernel (right for any lengths).
+ * head_dim 64 or 128; page strides and pools 16-byte aligned; scale positive. */
+int mt_attn_paged(const void* q, const void* k_pages, const void* v_pages, void* o, mt_strides3 sq, mt_strides3 spages,
+                  mt_strides3 so, const int32_t* tables, const int32_t* starts, const int32_t* kv_len,
+                  int64_t requests, int64_t width, int64_t rows, int64_t max_new, int64_t heads, int64_t kv_heads,
+                  int64_t head_dim, int64_t page_size, int64_t n_pages, float scale, int dtype, void* stream);
 
 /* ---- whole-model forward without a graph ----------------------------------
  * The inference branches of GPT2.forward (gpt2_trainer/gpt2.py:352-374) and of

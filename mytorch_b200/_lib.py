@@ -139,6 +139,10 @@ _SIG = {
     "mt_attn_decode": [_p, _p, _p, _p, _S, _S, _S, _i64, _i64, _i64, _i64, _i64, _f, _i, _i, _p],
     "mt_attn_decode_gqa": [_p, _p, _p, _p, _S, _S, _S, _i64, _i64, _i64, _i64, _i64, _i64, _f, _i, _i, _p],
     "mt_kv_append": [_p, _p, _p, _p, _S, _S, _S, _i64, _i64, _i64, _i64, _i64, _i64, _i, _p],
+    "mt_paged_tables": [_p] * 10 + [_i64] * 5 + [_p],
+    "mt_paged_release": [_p] * 5 + [_i64] * 4 + [_p],
+    "mt_paged_append": [_p, _p, _p, _p, _S, _S, _S, _p, _i64, _i64, _i64, _i64, _i64, _i, _p],
+    "mt_attn_paged": [_p, _p, _p, _p, _S, _S, _S, _p, _p, _p] + [_i64] * 9 + [_f, _i, _p],
     "mt_gpt_forward": [C.POINTER(GptModel), C.POINTER(GptPass), _p],
     "mt_argmax_rows": [_p, _p, _p, _i64, _i64, _i64, _i, _p],
     "mt_gradnorm_multi": [C.POINTER(TensorList), _i, _p, _p, _p, _p],

@@ -1,0 +1,65 @@
+// The paged key/value cache: what its kernels share (see mytorch_b200.h for the layout).
+#pragma once
+#include "common.cuh"
+
+namespace mt {
+
+constexpr int kPagedFlag = 3;            // device status: no page left, or a page or slot outside the pool
+
+// n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery, Division by Invariant Integers
+// using Multiplication, 1994): m = floor(2^32 (2^s - d) / d) + 1 with 2^s >= d.
+struct FastDiv {
+  uint32_t d, m, s;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t div) : d(div), s(0) {
+    while (s < 32 && (1ull << s) < div) ++s;
+    m = (uint32_t)((((1ull << s) - div) << 32) / div + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(m, n) + n) >> s; }
+};
+
+struct PagedAttnParams {
+  const void *q, *kp, *vp;
+  void* o;
+  mt_strides3 sq, sc, so;                // q, o: {-, head, row}; pools: {page, head, row}
+  const int32_t *tables, *starts, *kv_len;
+  int requests, width, rows, heads, kv_heads, group, n_pages;
+  FastDiv page, by_group;
+  float scale_log2;
+  int* flag;
+};
+
+// One request as the attention kernels see it. `past` may be negative (fewer keys than new rows: the
+// first rows see nothing).
+struct PagedRequest {
+  int q0, n_new, past, keys;
+};
+
+__device__ __forceinline__ PagedRequest paged_request(const PagedAttnParams& p, int r) {
+  const int a = p.starts[r], b = p.starts[r + 1], kv = p.kv_len[r];
+  PagedRequest x;
+  x.q0 = min(max(a, 0), p.rows);
+  x.n_new = min(max(b, x.q0), p.rows) - x.q0;
+  x.past = (int)max((int64_t)INT32_MIN / 2, (int64_t)kv - ((int64_t)b - a) + (x.q0 - (int64_t)a));
+  x.keys = (int)min((int64_t)max(kv, 0), (int64_t)p.width * p.page.d);
+  if (kv > x.keys && p.flag) atomicMax(p.flag, kPagedFlag);
+  return x;
+}
+
+// Number of keys that new row i of the request sees.
+__device__ __forceinline__ int visible_keys(const PagedRequest& x, int i) {
+  return (int)min((int64_t)x.keys, max((int64_t)0, (int64_t)x.past + i + 1));
+}
+
+// Element offset of a request's key row (for one head, add head * sc.h); -1 on a page outside the pool.
+__device__ __forceinline__ int64_t paged_row(const PagedAttnParams& p, const int32_t* table, int key) {
+  const uint32_t at = p.page.div((uint32_t)key);
+  const int page = table[at];
+  if ((unsigned)page >= (unsigned)p.n_pages) {
+    if (p.flag) atomicMax(p.flag, kPagedFlag);
+    return -1;
+  }
+  return (int64_t)page * p.sc.b + (int64_t)(key - (int)at * (int)p.page.d) * p.sc.s;
+}
+
+}  // namespace mt

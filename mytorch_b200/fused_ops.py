@@ -373,4 +373,99 @@ def fused_rope_rmsnorm_backward(dyq, dyk, yq, yk, rstd_q, rstd_k, cos, sin):
     return dq, dk
 
 
+# ---------------------------------------------------- paged key/value cache ----
+def _ints(name, a, *shape):
+    """An int32 array of the given shape (None = any extent)."""
+    a = _A(a)
+    if a.dtype != "int32" or len(a.shape) != len(shape) or any(n is not None and n != m for n, m in zip(shape, a.shape)):
+        raise ValueError(f"{name}: int32 {list(shape)} expected, got {a.dtype} {list(a.shape)}")
+    return a
+
+
+def _pools(k_pages, v_pages):
+    k, v = _A(k_pages), _A(v_pages)
+    if k.ndim != 4 or k.shape != v.shape:
+        raise ValueError(f"pools of keys and values are [pages, kv_heads, page_size, head_dim] both, got {k.shape} and {v.shape}")
+    return k, v
+
+
+def _page_strides(a):
+    _, H, S, D = a.shape
+    return _lib.Strides3(H * S * D, S * D, D)
+
+
+def fused_paged_tables(held, fresh, tables, free_pages, n_free, page_size, rows=None, out=None):
+    """Block tables and slot maps of one step, on the device: held, fresh int32 [R], tables int32 [R, width]
+    (this step's pages are written into it), free_pages int32 [list_len] with n_free int32 [1] of them free,
+    taken from the end. -> (starts [R+1], kv_len [R], position [rows], slot [rows], n_free after the step [1]),
+    see mt_paged_tables; `rows` is the number of token rows to describe (at least sum(fresh), which the host
+    need not know exactly), `out` the five arrays to write."""
+    held, free_pages, n_free = _ints("held", held, None), _ints("free_pages", free_pages, None), _ints("n_free", n_free, 1)
+    R = held.shape[0]
+    fresh, tables = _ints("fresh", fresh, R), _ints("tables", tables, R, None)
+    if out is None:
+        if rows is None:
+            raise ValueError("the number of token rows is needed where no arrays for the result are given")
+        out = [DeviceArray.empty((n,), "int32") for n in (R + 1, R, rows, rows, 1)]
+    starts, kv_len, position, slot, left = out
+    starts, kv_len, position, left = _ints("starts", starts, R + 1), _ints("kv_len", kv_len, R), _ints("position", position, rows), _ints("left", left, 1)
+    slot = _ints("slot", slot, position.shape[0])
+    _lib.paged_tables(held.ptr, fresh.ptr, tables.ptr, free_pages.ptr, n_free.ptr, starts.ptr, kv_len.ptr, position.ptr, slot.ptr,
+                      left.ptr, R, tables.shape[1], page_size, free_pages.shape[0], position.shape[0], stream())
+    return starts, kv_len, position, slot, left
+
+
+def fused_paged_release(done, tables, kv_len, free_pages, n_free, page_size):
+    """Gives the pages of the requests with done[r] != 0 back to the list (in place, mt_paged_release)."""
+    done, free_pages, n_free = _ints("done", done, None), _ints("free_pages", free_pages, None), _ints("n_free", n_free, 1)
+    R = done.shape[0]
+    tables, kv_len = _ints("tables", tables, R, None), _ints("kv_len", kv_len, R)
+    _lib.paged_release(done.ptr, tables.ptr, kv_len.ptr, free_pages.ptr, n_free.ptr, R, tables.shape[1], page_size,
+                       free_pages.shape[0], stream())
+
+
+def fused_paged_append(k, v, k_pages, v_pages, slot, strides=None):
+    """Rows of k, v [N, Hkv, D] into their slots of the pools [pages, Hkv, page_size, D] (in place); negative
+    slots are skipped. `strides` (two Strides3, batch unused) reads views such as a fused projection."""
+    k, v = _A(k), _A(v)
+    k_pages, v_pages = _pools(k_pages, v_pages)
+    _check_float(k, v, k_pages, v_pages)
+    P, H, S, D = k_pages.shape
+    if k.ndim != 3 or k.shape != v.shape or k.shape[1:] != (H, D):
+        raise ValueError(f"new keys and values are [rows, {H}, {D}] both, got {k.shape} and {v.shape}")
+    slot = _ints("slot", slot, k.shape[0])
+    sk, sv = strides or (_lib.Strides3(0, D, H * D),) * 2
+    _lib.paged_append(k.ptr, v.ptr, k_pages.ptr, v_pages.ptr, sk, sv, _page_strides(k_pages), slot.ptr, k.shape[0], H, D, S, P,
+                      k.code, stream())
+
+
+def fused_paged_attention(q, k_pages, v_pages, tables, starts, kv_len, max_new=None, softmax_scale=None, out=None, strides=None):
+    """Attention of the new rows q [N, H, D], packed by `starts` [R+1], over the pages that `tables` [R, width]
+    lists: kv_len [R] keys per request, this step's among them, causal (mt_attn_paged; grouped-query where H is
+    a multiple of the pools' heads). -> o [N, H, D]; rows that no request has keep what `out` held (0 without
+    `out`). max_new: the most new rows of one request, where the caller knows it (it picks the kernel only).
+    `strides` (Strides3, batch unused) reads q as a view. Not differentiable: a cache holds no graph."""
+    q = _A(q)
+    k_pages, v_pages = _pools(k_pages, v_pages)
+    _check_float(q, k_pages, v_pages)
+    P, Hk, S, D = k_pages.shape
+    if q.ndim != 3 or q.shape[2] != D or q.shape[1] % Hk:
+        raise ValueError(f"q is [rows, heads, {D}] with a multiple of {Hk} heads, got {q.shape}")
+    N, H, _ = q.shape
+    kv_len = _ints("kv_len", kv_len, None)
+    R = kv_len.shape[0]
+    tables, starts = _ints("tables", tables, R, None), _ints("starts", starts, R + 1)
+    if out is None:
+        out = DeviceArray.zeros((N, H, D), q.dtype)
+    else:
+        out = _A(out)
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError(f"out is {q.dtype} {q.shape}, got {out.dtype} {out.shape}")
+    row = _lib.Strides3(0, D, H * D)
+    _lib.attn_paged(q.ptr, k_pages.ptr, v_pages.ptr, out.ptr, strides or row, _page_strides(k_pages), row, tables.ptr, starts.ptr,
+                    kv_len.ptr, R, tables.shape[1], N, N if max_new is None else max_new, H, Hk, D, S, P,
+                    float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(D), q.code, stream())
+    return out
+
+
 __all__ = [n for n in dir() if n.startswith("fused_")] + ["gemm"]
