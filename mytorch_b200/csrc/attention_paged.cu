@@ -1,42 +1,8 @@
 // Attention of every request's new rows over the pages of its key/value cache (mt_attn_paged).
-#include "paged.cuh"
+#include "attention_paged.cuh"
+#include "paged_work.cuh"
 
 namespace mt {
-
-// One output row (a token's head) by one warp, straight from the definition: lane l holds D/32
-// neighbouring elements of q and o, scores are fp32 dot products, and only the visible keys are touched.
-template <typename T, int D>
-__device__ __forceinline__ void paged_row_plain(const PagedAttnParams& p, const PagedRequest& x, int r, int i, int h) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t head = (int64_t)(h / p.group) * p.sc.h;
-  const T* kp = (const T*)p.kp + head + lane * E;
-  const T* vp = (const T*)p.vp + head + lane * E;
-  const T* qp = (const T*)p.q + (int64_t)(x.q0 + i) * p.sq.s + (int64_t)h * p.sq.h + lane * E;
-  const int32_t* table = p.tables + (int64_t)r * p.width;
-  float q[E], o[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) { q[e] = to_f(qp[e]) * p.scale_log2; o[e] = 0.f; }
-  const int n = visible_keys(x, i);
-  for (int j = 0; j < n; ++j) {
-    const int64_t at = paged_row(p, table, j);
-    if (at < 0) continue;
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(q[e], to_f(kp[at + e]), s);
-    s = warp_sum(s);
-    const float mn = fmaxf(m, s);
-    if (mn == -INFINITY && !isnan(s)) continue;      // no finite score yet
-    const float c = m == -INFINITY ? 0.f : exp2f(m - mn), w = exp2f(s - (mn == -INFINITY ? 0.f : mn));
-    m = mn;
-    l = l * c + w;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(w, to_f(vp[at + e]), o[e] * c);
-  }
-  T* op = (T*)p.o + (int64_t)(x.q0 + i) * p.so.s + (int64_t)h * p.so.h + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; ++e) op[e] = from_f<T>(l == 0.f ? 0.f : o[e] / l);
-}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(128)
@@ -94,6 +60,8 @@ int mt_attn_paged(const void* q, const void* k_pages, const void* v_pages, void*
   p.scale_log2 = scale * 1.4426950408889634f;
   p.flag = device_flag_ptr();
   cudaStream_t st = as_stream(stream);
+  const int64_t row_hint = (max_new < rows ? max_new : rows) * p.group;
+  if (row_hint <= (dtype == MT_F32 ? 8 : 16)) return attn_paged_few(p, row_hint, (int)head_dim, dtype, st);
   MT_DISPATCH_FLOAT(dtype, T, return head_dim == 64 ? (launch_plain<T, 64>(p, st)) : (launch_plain<T, 128>(p, st)));
   return MT_OK;
 }

@@ -1,0 +1,307 @@
+// How attention over pages is shared out. Its work is a list of items - (request, key/value head, tile of
+// M query rows), a row being a (new token, query head of the group) pair - and an item is a run of key
+// tiles of KT keys. The host knows neither lengths nor how many items there are, and lengths differ
+// by orders of magnitude, so every block finds its own share on the device: the items, each weighted with the
+// keys its rows see, are laid end to end and cut into equal parts, one per block. A cut may fall inside an
+// item, at a key tile; the blocks on both sides then leave partial results (unnormalised output, maximum
+// and sum per row) that a second kernel joins in the order of the keys, so results do not depend on timing.
+#pragma once
+#include "paged.cuh"
+
+namespace mt {
+
+constexpr int kItemKeys = 64;            // an item's fixed cost (queries in, output out), in keys
+
+struct WorkPos { int r, hk, t, kt; };    // a key tile of an item; kt > 0: a cut inside the item
+
+__device__ __forceinline__ bool same_item(const WorkPos& a, const WorkPos& b) { return a.r == b.r && a.hk == b.hk && a.t == b.t; }
+
+template <int M>
+__device__ __forceinline__ int row_tiles(const PagedAttnParams& p, const PagedRequest& x) {
+  return (int)(((int64_t)x.n_new * p.group + M - 1) / M);
+}
+
+// Keys that the last row of tile t sees.
+template <int M>
+__device__ __forceinline__ int tile_keys(const PagedAttnParams& p, const PagedRequest& x, int t) {
+  const int64_t rows = min((int64_t)(t + 1) * M, (int64_t)x.n_new * p.group);
+  return visible_keys(x, (int)p.by_group.div((uint32_t)(rows - 1)));
+}
+
+// Weight of the first T of nt tiles of one head: closed form, increasing.
+template <int M>
+__device__ __forceinline__ int64_t weight_upto(const PagedAttnParams& p, const PagedRequest& x, int T, int nt) {
+  if (T == 0) return 0;
+  const int64_t base = max(x.past, 0) + kItemKeys;
+  const int64_t n = T < nt ? T : nt - 1;
+  const int64_t w = n * base + (int64_t)M * n * (n + 1) / 2 / p.group;
+  return T < nt ? w : w + base + x.n_new;
+}
+
+// Exclusive prefix sum of one value per thread and the block's total. `sh`: 33 values.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (int)blockDim.x >> 5;
+  int64_t s = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t t = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += t;
+  }
+  if (lane == 31) sh[warp] = s;
+  __syncthreads();
+  int64_t before = 0;
+  total = 0;
+  for (int w = 0; w < warps; ++w) {
+    if (w < warp) before += sh[w];
+    total += sh[w];
+  }
+  return s - v + before;
+}
+
+struct WorkShare { WorkPos begin, end; int blocks; };    // blocks that have work
+
+// This block's share; every thread calls it and gets the same answer. `min_weight`: at least so much per block.
+template <int M, int KT>
+__device__ __forceinline__ WorkShare find_share(const PagedAttnParams& p, int64_t min_weight) {
+  __shared__ int64_t sums[33];
+  __shared__ WorkPos found[2];
+  const int per = (p.requests + (int)blockDim.x - 1) / (int)blockDim.x;
+  const int r0 = min(p.requests, (int)threadIdx.x * per), r1 = min(p.requests, r0 + per);
+  auto weight = [&](const PagedRequest& x) { const int nt = row_tiles<M>(p, x); return weight_upto<M>(p, x, nt, nt) * p.kv_heads; };
+  int64_t mine = 0, total;
+  for (int r = r0; r < r1; ++r) mine += weight(paged_request(p, r));
+  if (threadIdx.x < 2) found[threadIdx.x] = WorkPos{p.requests, 0, 0, 0};
+  int64_t at = block_scan(mine, sums, total);
+  const int64_t many = total / min_weight;
+  const int blocks = (int)max((int64_t)1, min((int64_t)gridDim.x, many));
+  const int64_t share = total / blocks;
+  const int snap = (int)min((int64_t)INT32_MAX / 2, share / 8 / KT);    // cuts this near to an item's ends move there
+  for (int e = 0; e < 2; ++e) {
+    const int c = (int)blockIdx.x + e;
+    if (c >= blocks) continue;                       // the list's end
+    int64_t cut = (int64_t)((double)total * c / blocks);
+    if (cut < at || cut >= at + mine) continue;
+    cut -= at;
+    for (int r = r0; r < r1; ++r) {
+      const PagedRequest x = paged_request(p, r);
+      const int64_t w = weight(x);
+      if (cut >= w) { cut -= w; continue; }
+      const int nt = row_tiles<M>(p, x);
+      const int64_t head = weight_upto<M>(p, x, nt, nt);
+      WorkPos f;
+      f.r = r;
+      f.hk = (int)(cut / head);
+      cut -= f.hk * head;
+      int lo = 0, hi = nt;                           // the last tile that begins at or before the cut
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (weight_upto<M>(p, x, mid, nt) <= cut) lo = mid; else hi = mid;
+      }
+      const int64_t begin = weight_upto<M>(p, x, lo, nt), width = weight_upto<M>(p, x, lo + 1, nt) - begin;
+      const int n = (tile_keys<M>(p, x, lo) + KT - 1) / KT;
+      const int kt = (int)((double)(cut - begin) * n / width);
+      f.t = lo;
+      f.kt = kt <= snap ? 0 : kt;
+      if (f.kt && n - kt <= snap) { ++f.t; f.kt = 0; }
+      found[e] = f;
+      break;
+    }
+  }
+  __syncthreads();
+  WorkShare s;
+  s.begin = found[0];
+  s.end = found[1];
+  s.blocks = blocks;
+  if ((int)blockIdx.x >= blocks) s.begin = s.end;
+  return s;
+}
+
+struct WorkItem {
+  int r, hk, t;
+  int k0, k1, n;                         // key tiles [k0, k1) of n
+  int rows;                              // of the tile
+  int keys;                              // that its last row sees
+  PagedRequest x;
+};
+
+// Walks a share item by item.
+template <int M, int KT>
+struct WorkIter {
+  WorkPos cur, end;
+  int loaded, nt;
+  PagedRequest x;
+  __device__ __forceinline__ void start(const WorkShare& s) { cur = s.begin; end = s.end; loaded = -1; nt = 0; }
+  __device__ __forceinline__ bool next(const PagedAttnParams& p, WorkItem& it) {
+    for (;;) {
+      if (cur.r >= p.requests) return false;
+      if (cur.r > end.r || (cur.r == end.r && (cur.hk > end.hk || (cur.hk == end.hk && (cur.t > end.t || (cur.t == end.t && cur.kt >= end.kt))))))
+        return false;
+      if (loaded != cur.r) {
+        x = paged_request(p, cur.r);
+        nt = row_tiles<M>(p, x);
+        loaded = cur.r;
+      }
+      if (cur.t < nt) break;
+      cur.t = cur.kt = 0;
+      if (nt == 0 || ++cur.hk == p.kv_heads) { cur.hk = 0; ++cur.r; }
+    }
+    it.r = cur.r; it.hk = cur.hk; it.t = cur.t; it.x = x;
+    it.rows = (int)min((int64_t)M, (int64_t)x.n_new * p.group - (int64_t)cur.t * M);
+    it.keys = tile_keys<M>(p, x, cur.t);
+    it.n = (it.keys + KT - 1) / KT;
+    it.k0 = cur.kt;
+    it.k1 = same_item(cur, end) ? min(end.kt, it.n) : it.n;
+    ++cur.t;
+    cur.kt = 0;
+    return true;
+  }
+};
+
+// Partial results of a block's first and last item, where a cut runs through them: [2 per block][M rows]
+// of D sums, then the rows' maxima (log2 domain) and weights' sums; `cuts`: where every block begins, the number of
+// blocks with work behind the last.
+struct WorkPartials {
+  float* o;
+  float* ml;
+  WorkPos* cuts;
+};
+
+__device__ __forceinline__ int partial_slot(const WorkItem& it) {
+  return it.k0 > 0 ? 2 * (int)blockIdx.x : it.k1 < it.n ? 2 * (int)blockIdx.x + 1 : -1;
+}
+
+inline size_t partial_bytes(int blocks, int M, int D) {
+  return (size_t)blocks * 2 * M * (D + 2) * sizeof(float) + (size_t)(blocks + 1) * sizeof(WorkPos);
+}
+inline WorkPartials partials_in(void* buf, int blocks, int M, int D) {
+  WorkPartials w;
+  w.o = (float*)buf;
+  w.ml = w.o + (size_t)blocks * 2 * M * D;
+  w.cuts = (WorkPos*)(w.ml + (size_t)blocks * 2 * M * 2);
+  return w;
+}
+
+// The block whose share begins at blockIdx.x tells the joining kernel so.
+__device__ __forceinline__ void publish_share(const WorkShare& s, const WorkPartials& w) {
+  if (threadIdx.x == 0) {
+    w.cuts[blockIdx.x] = s.begin;
+    if (blockIdx.x == 0) w.cuts[gridDim.x] = WorkPos{s.blocks, 0, 0, 0};
+  }
+}
+
+// Token and query head of row `row` of an item's tile.
+template <int M>
+__device__ __forceinline__ void row_of(const PagedAttnParams& p, const WorkItem& it, int row, int& token, int& head) {
+  const uint32_t at = (uint32_t)it.t * M + row;
+  token = (int)p.by_group.div(at);
+  head = it.hk * p.group + (int)(at - (uint32_t)token * p.group);
+}
+
+// One output row (a token's head) by one warp, straight from the definition: lane l holds D/32
+// neighbouring elements of q and o, scores are fp32 dot products, and only the visible keys are touched.
+// The tiled kernels' masks are weights of zero, which a value that is not finite turns into NaN; rows
+// that come out as NaN are therefore computed again here.
+template <typename T, int D>
+__device__ __noinline__ void paged_row_plain(const PagedAttnParams& p, PagedRequest x, int r, int i, int h) {
+  constexpr int E = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t head = (int64_t)(h / p.group) * p.sc.h;
+  const T* kp = (const T*)p.kp + head + lane * E;
+  const T* vp = (const T*)p.vp + head + lane * E;
+  const T* qp = (const T*)p.q + (int64_t)(x.q0 + i) * p.sq.s + (int64_t)h * p.sq.h + lane * E;
+  const int32_t* table = p.tables + (int64_t)r * p.width;
+  float q[E], o[E], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) { q[e] = to_f(qp[e]) * p.scale_log2; o[e] = 0.f; }
+  const int n = visible_keys(x, i);
+  for (int j = 0; j < n; ++j) {
+    const int64_t at = paged_row(p, table, j);
+    if (at < 0) continue;
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) s = fmaf(q[e], to_f(kp[at + e]), s);
+    s = warp_sum(s);
+    const float mn = fmaxf(m, s);
+    if (mn == -INFINITY && !isnan(s)) continue;      // no finite score yet
+    const float c = m == -INFINITY ? 0.f : exp2f(m - mn), w = exp2f(s - (mn == -INFINITY ? 0.f : mn));
+    m = mn;
+    l = l * c + w;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = fmaf(w, to_f(vp[at + e]), o[e] * c);
+  }
+  T* op = (T*)p.o + (int64_t)(x.q0 + i) * p.so.s + (int64_t)h * p.so.h + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) op[e] = from_f<T>(l == 0.f ? 0.f : o[e] / l);
+}
+
+// Joins the partial results of the items that cuts run through: block (c, y) takes the item whose first cut
+// is the one between blocks c - 1 and c, a warp one row at a time. The pieces are weighted in the order of
+// the keys.
+template <typename T, int D, int M, int KT>
+__global__ void __launch_bounds__(128)
+paged_join_kernel(const PagedAttnParams p, const WorkPartials w, int grid) {
+  constexpr int E = D / 32;
+  grid_dependency_wait();
+  const int blocks = w.cuts[grid].r, c = (int)blockIdx.x + 1;
+  if (c >= blocks) return;
+  const WorkPos cut = w.cuts[c], before = w.cuts[c - 1];
+  if (cut.kt == 0 || (before.kt > 0 && same_item(before, cut))) return;
+  int last = c;                                      // the item's pieces: slot 2c-1, then 2j of blocks c..last
+  while (last + 1 < blocks && same_item(w.cuts[last + 1], cut) && w.cuts[last + 1].kt > 0) ++last;
+  const int pieces = last - c + 2;
+  WorkItem it;
+  it.r = cut.r; it.hk = cut.hk; it.t = cut.t;
+  it.x = paged_request(p, cut.r);
+  it.rows = (int)min((int64_t)M, (int64_t)it.x.n_new * p.group - (int64_t)cut.t * M);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // an empty piece (two cuts at one key tile) was not written
+  auto slot_of = [&](int i) {
+    if (i == 0) return 2 * (c - 1) + 1;
+    const int j = c + i - 1;
+    return j < last && w.cuts[j + 1].kt == w.cuts[j].kt ? -1 : 2 * j;
+  };
+  for (int row = (int)blockIdx.y * 4 + warp; row < it.rows; row += 4 * gridDim.y) {
+    float m = -INFINITY;
+    for (int i = lane; i < pieces; i += 32) {
+      const int s = slot_of(i);
+      if (s >= 0) m = fmaxf(m, w.ml[((int64_t)s * M + row) * 2]);
+    }
+    m = warp_max(m);
+    float l = 0.f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < pieces; ++i) {
+      const int s = slot_of(i);
+      if (s < 0) continue;
+      const float* ml = w.ml + ((int64_t)s * M + row) * 2;
+      const float a = ml[0] == -INFINITY ? (isnan(ml[1]) ? ml[1] : 0.f) : exp2f(ml[0] - m);
+      l = fmaf(ml[1], a, l);
+      const float* src = w.o + ((int64_t)s * M + row) * D + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(src[e], a, o[e]);
+    }
+    int token, head;
+    row_of<M>(p, it, row, token, head);
+    bool nan = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) { o[e] = l == 0.f ? 0.f : o[e] / l; nan |= isnan(o[e]); }
+    if (__any_sync(0xffffffffu, nan)) {
+      paged_row_plain<T, D>(p, it.x, it.r, token, head);
+      continue;
+    }
+    T* op = (T*)p.o + (int64_t)(it.x.q0 + token) * p.so.s + (int64_t)head * p.so.h + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) op[e] = from_f<T>(o[e]);
+  }
+}
+
+template <typename T, int D, int M, int KT>
+static int launch_join(const PagedAttnParams& p, const WorkPartials& w, int grid, cudaStream_t st) {
+  if (grid < 2) return MT_OK;
+  MT_CHECK_CUDA(launch_overlapped(paged_join_kernel<T, D, M, KT>, dim3((unsigned)grid - 1, M >= 64 ? M / 16 : (M + 3) / 4), dim3(128), 0, st, p, w, grid));
+  count_launch();
+  return MT_OK;
+}
+
+}  // namespace mt
