@@ -62,6 +62,7 @@ int mt_attn_paged(const void* q, const void* k_pages, const void* v_pages, void*
   cudaStream_t st = as_stream(stream);
   const int64_t row_hint = (max_new < rows ? max_new : rows) * p.group;
   if (row_hint <= (dtype == MT_F32 ? 8 : 16)) return attn_paged_few(p, row_hint, (int)head_dim, dtype, st);
+  if (dtype != MT_F32) return attn_paged_tc(p, (int)head_dim, dtype, st);
   MT_DISPATCH_FLOAT(dtype, T, return head_dim == 64 ? (launch_plain<T, 64>(p, st)) : (launch_plain<T, 128>(p, st)));
   return MT_OK;
 }

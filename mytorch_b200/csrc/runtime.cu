@@ -63,6 +63,21 @@ int sm_count() {
   return g_sms[dev];
 }
 
+// The device's pool keeps what is freed: without that every allocation after a synchronisation maps
+// memory anew (120 us).
+int ensure_pool() {
+  int dev = 0;
+  MT_CHECK_CUDA(cudaGetDevice(&dev));
+  if (dev < kMaxDev && !g_pool_ready[dev]) {
+    cudaMemPool_t pool;
+    MT_CHECK_CUDA(cudaDeviceGetDefaultMemPool(&pool, dev));
+    uint64_t thr = UINT64_MAX;  // keep freed blocks cached in the pool
+    MT_CHECK_CUDA(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &thr));
+    g_pool_ready[dev] = true;
+  }
+  return MT_OK;
+}
+
 // ---- timing of one kernel class --------------------------------------------
 static int g_prof_kind = 0;
 struct ProfRec { cudaEvent_t a, b; double flops; };
@@ -119,19 +134,6 @@ int mt_device_count(int* count) {
 int mt_set_device(int device) { MT_CHECK_CUDA(cudaSetDevice(device)); return MT_OK; }
 int mt_get_device(int* device) { MT_CHECK_CUDA(cudaGetDevice(device)); return MT_OK; }
 int mt_device_sm_count(int* count) { *count = sm_count(); return MT_OK; }
-
-static int ensure_pool() {
-  int dev = 0;
-  MT_CHECK_CUDA(cudaGetDevice(&dev));
-  if (dev < kMaxDev && !g_pool_ready[dev]) {
-    cudaMemPool_t pool;
-    MT_CHECK_CUDA(cudaDeviceGetDefaultMemPool(&pool, dev));
-    uint64_t thr = UINT64_MAX;  // keep freed blocks cached in the pool
-    MT_CHECK_CUDA(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &thr));
-    g_pool_ready[dev] = true;
-  }
-  return MT_OK;
-}
 
 int mt_malloc(void** ptr, size_t bytes, void* stream) {
   *ptr = nullptr;

@@ -6,12 +6,15 @@
 #include "common.cuh"
 
 namespace mt {
+int ensure_pool();   // the current device's pool keeps what is freed
+
 struct TempBuf {
   void* ptr = nullptr;
   cudaStream_t st;
   bool ok_ = true;
   TempBuf(size_t bytes, cudaStream_t s) : st(s) {
     if (bytes == 0) return;
+    if (ensure_pool() != MT_OK) { ok_ = false; return; }
     cudaError_t e = cudaMallocAsync(&ptr, bytes, s);
     if (e != cudaSuccess) {
       set_error("scratch allocation of %zu bytes failed: %s", bytes, cudaGetErrorString(e));
