@@ -6,7 +6,7 @@ namespace mt {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(128)
-paged_plain_kernel(const PagedAttnParams p) {
+paged_plain_kernel(const __grid_constant__ PagedAttnParams p) {
   const int64_t at = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int token = (int)(at / p.heads), h = (int)(at % p.heads);
   if (token >= p.rows || token < p.starts[0] || token >= p.starts[p.requests]) return;
@@ -58,10 +58,15 @@ int mt_attn_paged(const void* q, const void* k_pages, const void* v_pages, void*
   p.group = (int)(heads / kv_heads); p.n_pages = (int)n_pages;
   p.page = FastDiv((uint32_t)page_size); p.by_group = FastDiv((uint32_t)p.group);
   p.scale_log2 = scale * 1.4426950408889634f;
+  auto on = [&](const void* x, mt_strides3 t, int64_t elems) {
+    return (uintptr_t)x % (elems * dtype_size(dtype)) == 0 && t.h % elems == 0 && t.s % elems == 0;
+  };
+  p.q_pairs = on(q, sq, 2);
+  p.o_quads = on(o, so, 4);
   p.flag = device_flag_ptr();
   cudaStream_t st = as_stream(stream);
   const int64_t row_hint = (max_new < rows ? max_new : rows) * p.group;
-  if (row_hint <= (dtype == MT_F32 ? 8 : 16)) return attn_paged_few(p, row_hint, (int)head_dim, dtype, st);
+  if (row_hint <= (dtype == MT_F32 ? 8 : 32)) return attn_paged_few(p, row_hint, (int)head_dim, dtype, st);
   if (dtype != MT_F32) return attn_paged_tc(p, (int)head_dim, dtype, st);
   MT_DISPATCH_FLOAT(dtype, T, return head_dim == 64 ? (launch_plain<T, 64>(p, st)) : (launch_plain<T, 128>(p, st)));
   return MT_OK;

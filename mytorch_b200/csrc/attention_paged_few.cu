@@ -1,40 +1,47 @@
 // Attention over pages for few query rows per key/value head: decoding steps and a few drafted tokens.
 //
 // HBM bound: every key and value row of a head is read once (2 D bytes a key in half precision, against
-// 4 D operations per query row). A block of four warps works on one item at a time: up to 16 rows (tokens times the query
-// heads of the group) and a run of key tiles. A warp owns 16 keys (8 in fp32) of each tile and has a ring
-// of stages of its own, filled by 16-byte cp.async: page lookups run one tile ahead of the loads,
+// 4 D operations per query row). A block of four warps works on one item at a time: M rows (tokens times the
+// query heads of the group) and a run of key tiles. A warp owns a part of each tile (16 or 32 keys, 8 in fp32)
+// and has a ring of stages of its own, filled by 16-byte cp.async: page lookups run one tile ahead of the loads,
 // loads up to three tiles ahead of the products and on across item boundaries, and no warp waits for
 // another until an item's end. Rows that are not there (behind the last key, on a bad page) are
 // filled with zeros and masked, so whatever lies in unused rows of a page is never read.
-//   half: S = Q K^T and O += P V by mma.sync (m16n8k16). The tensor pipe is idle otherwise (2 % busy), so 1 to 16 rows cost
-//         the same, and P goes in as a pair of halves (rounded value and remainder): the weights keep about
-//         fp32's precision and the output is as exact as one rounding allows.
+//   half: transposed products by mma.sync (m16n8k16), S^T = K Q^T and O^T += V^T P^T, so that the keys fill
+//         the 16 rows of an MMA and the queries are its 8 columns: with one to eight rows per item (decoding) half the products,
+//         registers and exponentials of the other way round. P^T moves from accumulators to operands by
+//         movmatrix, as a pair of halves (rounded value and remainder): the tensor pipe has room, the weights
+//         keep about fp32's precision, and the output is as exact as one rounding allows.
 //   fp32: lane = key and quarter of head_dim for the scores, lane = elements of head_dim for the output.
 // The online softmax is kept per warp; warps join at an item's end through shared memory, blocks through
 // the partial results of paged_work.cuh.
 #include "attention_paged.cuh"
 #include "paged_work.cuh"
 #include "tempbuf.cuh"
-#include <type_traits>
 
 namespace mt {
 
 constexpr int kFewWarps = 4;
 
+// M rows per item: 8, 16, 24 or 32 in half precision, 1, 2, 4 or 8 in fp32.
 template <typename T, int D, int M> struct FewCfg {
   static constexpr bool kHalf = sizeof(T) == 2;
-  static constexpr int kRows = kHalf ? 16 : 8;                   // keys of a warp in a tile
+  static constexpr int kRows = kHalf ? (D == 64 ? 32 : 16) : 8;  // keys of a warp in a tile
   static constexpr int KT = kRows * kFewWarps;
   static constexpr int kChunks = D * (int)sizeof(T) / 16;        // 16-byte pieces of a row
   static constexpr int kTile = kRows * kChunks * 16;             // bytes of a warp's keys (or values) of one tile
-  static constexpr int kStages = !kHalf && M == 8 && D == 128 ? 2 : 3;
+  static constexpr int kStages = kHalf ? 2 : M == 8 && D == 128 ? 2 : 3;
   static constexpr int kRing = kStages * 2 * kTile;              // per warp
+  static constexpr int kPitch = D + 4;                           // of a row of results in shared memory, floats
+  static constexpr int kParts = kHalf ? 2 : kFewWarps;           // results that meet there
   static constexpr int kOffMerge = kFewWarps * kRing;
-  static constexpr int kMerge = (kHalf ? 2 : kFewWarps) * M * D * 4;
-  static constexpr int kOffQ = kOffMerge + kMerge;               // fp32: the scaled queries
-  static constexpr int kOffStat = kOffQ + (kHalf ? 0 : M * D * 4);
+  static constexpr int kOffQ = kOffMerge + kParts * M * kPitch * 4;   // fp32: the scaled queries
+  static constexpr int kOffStat = kOffQ + (kHalf ? 0 : M * D * 4);    // maxima and sums, [2][warps][M]
   static constexpr int kSmem = kOffStat + kFewWarps * M * 2 * 4 + kFewWarps * kStages * 4;
+  // 228 KB per SM, of which every block costs 1 KB and 336 bytes of static shared memory besides its own
+  static constexpr int kFit = 233472 / (kSmem + 1024 + 336);
+  static constexpr int kBlocks = kFit < (kHalf ? 3 : 4) ? kFit : (kHalf ? 3 : 4);
+  static_assert(kBlocks >= 2, "two blocks per SM");
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -61,6 +68,12 @@ template <> __device__ __forceinline__ void mma16<__half>(float (&c)[4], const u
 template <> __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Transposes an 8x8 matrix of halves held as one pair per lane.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 template <typename T> __device__ __forceinline__ uint32_t pair_bits(T a, T b) {
   return (uint32_t)*reinterpret_cast<uint16_t*>(&a) | (uint32_t)*reinterpret_cast<uint16_t*>(&b) << 16;
@@ -107,7 +120,7 @@ struct FewLoader {
       const int key = kt * Cfg::KT + warp * Cfg::kRows + (lane % Cfg::kRows);
       const uint32_t in_page = (uint32_t)key - p.page.div((uint32_t)key) * p.page.d;
       const int64_t off = page >= 0 ? (int64_t)page * p.sc.b + (int64_t)in_page * p.sc.s + (int64_t)it.hk * p.sc.h : -1;
-      const uint32_t mask = __ballot_sync(0xffffffffu, off >= 0) & ((1u << Cfg::kRows) - 1);
+      const uint32_t mask = __ballot_sync(0xffffffffu, off >= 0) & (uint32_t)((1ull << Cfg::kRows) - 1);
       if (lane == 0) masks[stage] = mask;
       if (mask) {
         const uint32_t kd = ring + stage * 2 * Cfg::kTile, vd = kd + Cfg::kTile;
@@ -128,14 +141,57 @@ struct FewLoader {
   }
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kFewWarps * 32, 2)
-paged_few_half_kernel(const PagedAttnParams p, const WorkPartials w, int64_t min_weight) {
-  constexpr int M = 16;
+// An item's results, from `Cfg::kParts` parts in shared memory, weighted by `factor(part, row)`: to the output, or to
+// the block's partial results. top, sum: of a row.
+template <typename T, int D, int M, typename Cfg, typename Row, typename Factor>
+__device__ __forceinline__ void few_finish(const PagedAttnParams& p, const WorkPartials& w, const WorkItem& it, const float* merge,
+                                           Row row_stats, Factor factor) {
+  constexpr int E = D / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slot = partial_slot(it);
+  for (int g = warp; g < it.rows; g += kFewWarps) {
+    float top, sum, o[E];
+    row_stats(g, top, sum);
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll
+    for (int v = 0; v < Cfg::kParts; ++v) {
+      const float f = factor(v, g, top);
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(merge[(v * M + g) * Cfg::kPitch + lane * E + e], f, o[e]);
+    }
+    if (slot >= 0) {
+      struct alignas(4 * E) Pack { float t[E]; } pack;
+#pragma unroll
+      for (int e = 0; e < E; ++e) pack.t[e] = o[e];
+      *reinterpret_cast<Pack*>(w.o + ((int64_t)slot * M + g) * D + lane * E) = pack;
+      if (lane == 0) *reinterpret_cast<float2*>(w.ml + ((int64_t)slot * M + g) * 2) = make_float2(top, sum);
+      continue;
+    }
+    int token, head;
+    row_of<M>(p, it, g, token, head);
+    bool nan = false;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int e = 0; e < E; ++e) { o[e] *= inv; nan |= isnan(o[e]); }
+    if (__any_sync(0xffffffffu, nan)) paged_row_plain<T, D>(p, it.x, it.r, token, head);
+    else store_row<T, E>(p, it.x, token, head, o);
+  }
+}
+
+// The weight of a part with maximum m and sum l where the maximum of all is `top`. Without a maximum there are no
+// weights, or only NaN ones, which stay.
+__device__ __forceinline__ float part_weight(float m, float l, float top) {
+  return m == -INFINITY ? (isnan(l) ? l : 0.f) : exp2f(m - top);
+}
+
+template <typename T, int D, int M>
+__global__ void __launch_bounds__(kFewWarps * 32, FewCfg<T, D, M>::kBlocks)
+paged_few_half_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w, int min_weight) {
   using Cfg = FewCfg<T, D, M>;
+  constexpr int NT = M / 8, KM = Cfg::kRows / 16, C = Cfg::kChunks;
   extern __shared__ __align__(128) uint8_t few_smem[];
   float* merge = reinterpret_cast<float*>(few_smem + Cfg::kOffMerge);
-  float* stat = reinterpret_cast<float*>(few_smem + Cfg::kOffStat);            // [warps][16] maxima, then sums
+  float* stat = reinterpret_cast<float*>(few_smem + Cfg::kOffStat);            // [warps][M] maxima, then sums
   uint32_t* masks = reinterpret_cast<uint32_t*>(stat + kFewWarps * M * 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   allow_dependents();
@@ -151,27 +207,34 @@ paged_few_half_kernel(const PagedAttnParams p, const WorkPartials w, int64_t min
   iter.start(share);
   WorkItem it;
   int stage = 0;
+  const int quad = lane >> 2, pair = 2 * (lane & 3);     // a fragment's row (or column), and its first element along the other side
   while (iter.next(p, it)) {
-    const int ra = lane >> 2, rb = ra + 8;           // this thread's two rows
-    int lim_a = INT32_MAX, lim_b = INT32_MAX, tok, head;
-    uint32_t qf[D / 16][4];
-    row_of<M>(p, it, ra, tok, head);
-    const T* qa = (const T*)p.q + (int64_t)(it.x.q0 + tok) * p.sq.s + (int64_t)head * p.sq.h + 2 * (lane & 3);
-    if (ra < it.rows) lim_a = visible_keys(it.x, tok);
-    row_of<M>(p, it, rb, tok, head);
-    const T* qb = (const T*)p.q + (int64_t)(it.x.q0 + tok) * p.sq.s + (int64_t)head * p.sq.h + 2 * (lane & 3);
-    if (rb < it.rows) lim_b = visible_keys(it.x, tok);
+    uint32_t qf[NT][D / 16][2];                          // Q^T as the right operand: column = query row
+    int tok, head;
 #pragma unroll
-    for (int k = 0; k < D / 16; ++k) {
-      qf[k][0] = ra < it.rows ? pair_bits(qa[k * 16], qa[k * 16 + 1]) : 0u;
-      qf[k][1] = rb < it.rows ? pair_bits(qb[k * 16], qb[k * 16 + 1]) : 0u;
-      qf[k][2] = ra < it.rows ? pair_bits(qa[k * 16 + 8], qa[k * 16 + 9]) : 0u;
-      qf[k][3] = rb < it.rows ? pair_bits(qb[k * 16 + 8], qb[k * 16 + 9]) : 0u;
+    for (int n = 0; n < NT; ++n) {
+      const int row = 8 * n + quad;
+      row_of<M>(p, it, row, tok, head);
+      const bool real = row < it.rows;
+      const T* q = (const T*)p.q + (real ? (int64_t)(it.x.q0 + tok) * p.sq.s + (int64_t)head * p.sq.h + pair : 0);
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const T* at = q + k * 16 + h * 8;
+          qf[n][k][h] = !real ? 0u : p.q_pairs ? *reinterpret_cast<const uint32_t*>(at) : pair_bits(at[0], at[1]);
+        }
     }
-    float acc[D / 8][4], ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;
+    row_of<M>(p, it, 0, tok, head);
+    const int first_lim = visible_keys(it.x, tok);       // the tile's first row sees the fewest keys
+    float acc[NT][D / 16][4], m[NT][2], l[NT][2];
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-    const int first_lim = __shfl_sync(0xffffffffu, lim_a, 0);                  // the tile's first row sees the fewest keys
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) acc[n][d][0] = acc[n][d][1] = acc[n][d][2] = acc[n][d][3] = 0.f;
+    }
     for (int kt = it.k0; kt < it.k1; ++kt) {
       copy_wait<Cfg::kStages - 1>();
       __syncwarp();
@@ -179,174 +242,158 @@ paged_few_half_kernel(const PagedAttnParams p, const WorkPartials w, int64_t min
       const int key0 = kt * Cfg::KT + warp * Cfg::kRows;
       if (mask) {
         const uint32_t kb = load.ring + stage * 2 * Cfg::kTile, vb = kb + Cfg::kTile;
-        float s[2][4] = {};
+        float s[KM][NT][4];
+#pragma unroll
+        for (int i = 0; i < KM; ++i)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.f;
         {
-          const int row = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+          const int row = lane & 15, half = lane >> 4;
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            uint32_t b[4];
-            ldm4(b, kb + (row * Cfg::kChunks + ((2 * k + half) ^ (row & 7))) * 16);
-            mma16<T>(s[0], qf[k], b[0], b[1]);
-            mma16<T>(s[1], qf[k], b[2], b[3]);
-          }
-        }
-        const bool full = mask == 0xffffu && key0 + 16 <= first_lim;
-        float xa = ma, xb = mb;
+          for (int k = 0; k < D / 16; ++k)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+            for (int i = 0; i < KM; ++i) {
+              uint32_t a[4];
+              ldm4(a, kb + ((16 * i + row) * C + ((2 * k + half) ^ (row & 7))) * 16);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int j = n * 8 + 2 * (lane & 3) + e;
-            s[n][e] *= p.scale_log2;
-            s[n][2 + e] *= p.scale_log2;
-            if (!full) {
-              const bool there = (mask >> j) & 1;
-              if (!there || key0 + j >= lim_a) s[n][e] = -INFINITY;
-              if (!there || key0 + j >= lim_b) s[n][2 + e] = -INFINITY;
+              for (int n = 0; n < NT; ++n) mma16<T>(s[i][n], a, qf[n][k][0], qf[n][k][1]);
             }
-            xa = fmaxf(xa, s[n][e]);
-            xb = fmaxf(xb, s[n][2 + e]);
-          }
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-          xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, o));
-          xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, o));
         }
-        if (__any_sync(0xffffffffu, xa > ma || xb > mb)) {
-          const float ca = ma == -INFINITY ? 0.f : exp2f(ma - xa), cb = mb == -INFINITY ? 0.f : exp2f(mb - xb);
-          ma = xa;
-          mb = xb;
-          la *= ca;
-          lb *= cb;
+        const bool full = mask == (uint32_t)((1ull << Cfg::kRows) - 1) && key0 + Cfg::kRows <= first_lim;
+        if (!full) {
 #pragma unroll
-          for (int i = 0; i < D / 8; ++i) { acc[i][0] *= ca; acc[i][1] *= ca; acc[i][2] *= cb; acc[i][3] *= cb; }
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int row = 8 * n + pair + e;
+              row_of<M>(p, it, row, tok, head);
+              const int lim = row < it.rows ? visible_keys(it.x, tok) : 0;
+#pragma unroll
+              for (int i = 0; i < KM; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const int j = 16 * i + 8 * h + quad;
+                  if (!((mask >> j) & 1) || key0 + j >= lim) s[i][n][2 * h + e] = -INFINITY;
+                }
+            }
         }
-        const float ua = ma == -INFINITY ? 0.f : ma, ub = mb == -INFINITY ? 0.f : mb;
-        uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < NT; ++n) {
+          float x[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {              // row a, row b
-            const float p0 = exp2f(s[n][2 * b] - (b ? ub : ua)), p1 = exp2f(s[n][2 * b + 1] - (b ? ub : ua));
-            (b ? lb : la) += p0 + p1;
-            const T h0 = from_f<T>(p0), h1 = from_f<T>(p1);
-            hi[2 * n + b] = pair_bits(h0, h1);
-            lo[2 * n + b] = pair_bits(from_f<T>(p0 - to_f(h0)), from_f<T>(p1 - to_f(h1)));
+          for (int i = 0; i < KM; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) x[e] = fmaxf(x[e], s[i][n][2 * h + e]);
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+            x[0] = fmaxf(x[0], __shfl_xor_sync(0xffffffffu, x[0], o));
+            x[1] = fmaxf(x[1], __shfl_xor_sync(0xffffffffu, x[1], o));
           }
-        const int row = (lane & 7) + (((lane >> 3) & 1) << 3), next = lane >> 4;
+          x[0] = fmaxf(x[0] * p.scale_log2, m[n][0]);
+          x[1] = fmaxf(x[1] * p.scale_log2, m[n][1]);
+          if (__any_sync(0xffffffffu, x[0] > m[n][0] || x[1] > m[n][1])) {
+            const float c0 = m[n][0] == -INFINITY ? 0.f : exp2f(m[n][0] - x[0]), c1 = m[n][1] == -INFINITY ? 0.f : exp2f(m[n][1] - x[1]);
+            m[n][0] = x[0];
+            m[n][1] = x[1];
+            l[n][0] *= c0;
+            l[n][1] *= c1;
 #pragma unroll
-        for (int c = 0; c < D / 8; c += 2) {
-          uint32_t b[4];
-          ldm4t(b, vb + (row * Cfg::kChunks + ((c + next) ^ (row & 7))) * 16);
-          mma16<T>(acc[c], hi, b[0], b[1]);
-          mma16<T>(acc[c + 1], hi, b[2], b[3]);
-          mma16<T>(acc[c], lo, b[0], b[1]);
-          mma16<T>(acc[c + 1], lo, b[2], b[3]);
+            for (int d = 0; d < D / 16; ++d) { acc[n][d][0] *= c0; acc[n][d][1] *= c1; acc[n][d][2] *= c0; acc[n][d][3] *= c1; }
+          }
+          const float u0 = m[n][0] == -INFINITY ? 0.f : m[n][0], u1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+          uint32_t hi[KM][2], lo[KM][2];                 // P^T as the right operand
+#pragma unroll
+          for (int i = 0; i < KM; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float p0 = exp2f(fmaf(s[i][n][2 * h], p.scale_log2, -u0)), p1 = exp2f(fmaf(s[i][n][2 * h + 1], p.scale_log2, -u1));
+              l[n][0] += p0;
+              l[n][1] += p1;
+              const T h0 = from_f<T>(p0), h1 = from_f<T>(p1);
+              hi[i][h] = transpose8(pair_bits(h0, h1));
+              lo[i][h] = transpose8(pair_bits(from_f<T>(p0 - to_f(h0)), from_f<T>(p1 - to_f(h1))));
+            }
+          const int row = (lane & 7) + ((lane >> 4) << 3), next = (lane >> 3) & 1;
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+            for (int i = 0; i < KM; ++i) {
+              uint32_t a[4];
+              ldm4t(a, vb + ((16 * i + row) * C + ((2 * d + next) ^ (row & 7))) * 16);
+              mma16<T>(acc[n][d], a, hi[i][0], hi[i][1]);
+              mma16<T>(acc[n][d], a, lo[i][0], lo[i][1]);
+            }
         }
       }
       __syncwarp();
       load.issue(p, stage, warp, lane);
       stage = stage + 1 == Cfg::kStages ? 0 : stage + 1;
     }
-    // the warps' results: a common maximum, then sums of pairs of warps
+    // the warps' results: a common maximum, then warps 2 and 3 into 0 and 1, and those two in few_finish
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      la += __shfl_xor_sync(0xffffffffu, la, o);
-      lb += __shfl_xor_sync(0xffffffffu, lb, o);
-    }
-    if ((lane & 3) == 0) {
-      stat[warp * M + ra] = ma;
-      stat[warp * M + rb] = mb;
-      stat[(kFewWarps + warp) * M + ra] = la;
-      stat[(kFewWarps + warp) * M + rb] = lb;
-    }
-    __syncthreads();
-    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int v = 0; v < kFewWarps; ++v) {
-      top[0] = fmaxf(top[0], stat[v * M + ra]);
-      top[1] = fmaxf(top[1], stat[v * M + rb]);
-    }
-    // without a maximum there are no weights, or only NaN ones, which stay
-    auto factor = [](float m, float t, float l) { return m == -INFINITY ? (isnan(l) ? l : 0.f) : exp2f(m - t); };
+      for (int e = 0; e < 2; ++e) {
 #pragma unroll
-    for (int v = 0; v < kFewWarps; ++v) {
-      const float l0 = stat[(kFewWarps + v) * M + ra], l1 = stat[(kFewWarps + v) * M + rb];
-      sum[0] = fmaf(l0, factor(stat[v * M + ra], top[0], l0), sum[0]);
-      sum[1] = fmaf(l1, factor(stat[v * M + rb], top[1], l1), sum[1]);
-    }
-    const float fa = factor(ma, top[0], la), fb = factor(mb, top[1], lb);
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) { acc[i][0] *= fa; acc[i][1] *= fa; acc[i][2] *= fb; acc[i][3] *= fb; }
-    auto hand_over = [&](float* to) {
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float4*>(to + (i * 32 + lane) * 4) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
-    };
-    auto take_in = [&](const float* from) {
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        const float4 v = *reinterpret_cast<const float4*>(from + (i * 32 + lane) * 4);
-        acc[i][0] += v.x; acc[i][1] += v.y; acc[i][2] += v.z; acc[i][3] += v.w;
-      }
-    };
-    if (warp >= 2) hand_over(merge + (warp - 2) * M * D);
-    __syncthreads();
-    if (warp < 2) take_in(merge + warp * M * D);
-    __syncthreads();
-    if (warp == 1) hand_over(merge);
-    __syncthreads();
-    if (warp == 0) {
-      take_in(merge);
-      const int slot = partial_slot(it);
-      if (slot >= 0) {
-        float* po = w.o + (int64_t)slot * M * D;
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          *reinterpret_cast<float2*>(po + ra * D + i * 8 + 2 * (lane & 3)) = make_float2(acc[i][0], acc[i][1]);
-          *reinterpret_cast<float2*>(po + rb * D + i * 8 + 2 * (lane & 3)) = make_float2(acc[i][2], acc[i][3]);
-        }
-        if ((lane & 3) == 0) {
-          float* ml = w.ml + (int64_t)slot * M * 2;
-          *reinterpret_cast<float2*>(ml + 2 * ra) = make_float2(top[0], sum[0]);
-          *reinterpret_cast<float2*>(ml + 2 * rb) = make_float2(top[1], sum[1]);
-        }
-      } else {
-        const float ia = sum[0] == 0.f ? 0.f : 1.f / sum[0], ib = sum[1] == 0.f ? 0.f : 1.f / sum[1];
-        bool nan_a = false, nan_b = false;
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          acc[i][0] *= ia; acc[i][1] *= ia; acc[i][2] *= ib; acc[i][3] *= ib;
-          nan_a |= isnan(acc[i][0]) || isnan(acc[i][1]);
-          nan_b |= isnan(acc[i][2]) || isnan(acc[i][3]);
-        }
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const int row = b ? rb : ra;
-          row_of<M>(p, it, row, tok, head);
-          if (row < it.rows) {
-            T* op = (T*)p.o + (int64_t)(it.x.q0 + tok) * p.so.s + (int64_t)head * p.so.h + 2 * (lane & 3);
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) { op[i * 8] = from_f<T>(acc[i][2 * b]); op[i * 8 + 1] = from_f<T>(acc[i][2 * b + 1]); }
-          }
-          uint32_t again = __ballot_sync(0xffffffffu, b ? nan_b : nan_a);
-          while (again) {                            // rows with NaN, four lanes each
-            const int q = (__ffs((int)again) - 1) >> 2;
-            again &= ~(0xfu << (4 * q));
-            if (q + 8 * b >= it.rows) continue;
-            row_of<M>(p, it, q + 8 * b, tok, head);
-            __syncwarp();
-            paged_row_plain<T, D>(p, it.x, it.r, tok, head);
-          }
+        for (int o = 4; o < 32; o <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o);
+        if (quad == 0) {
+          stat[warp * M + 8 * n + pair + e] = m[n][e];
+          stat[(kFewWarps + warp) * M + 8 * n + pair + e] = l[n][e];
         }
       }
+    __syncthreads();
+    auto row_stats = [&](int g, float& top, float& sum) {
+      top = -INFINITY;
+      sum = 0.f;
+#pragma unroll
+      for (int v = 0; v < kFewWarps; ++v) top = fmaxf(top, stat[v * M + g]);
+#pragma unroll
+      for (int v = 0; v < kFewWarps; ++v) {
+        const float lv = stat[(kFewWarps + v) * M + g];
+        sum = fmaf(lv, part_weight(stat[v * M + g], lv, top), sum);
+      }
+    };
+    auto part = [&](int v, int n, int d, int i) -> float& {   // element i of a fragment in part v
+      return merge[(v * M + 8 * n + pair + (i & 1)) * Cfg::kPitch + 16 * d + 8 * (i >> 1) + quad];
+    };
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float f[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float top, sum;
+        row_stats(8 * n + pair + e, top, sum);
+        f[e] = part_weight(m[n][e], l[n][e], top);
+      }
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc[n][d][i] *= f[i & 1];
+          if (warp >= 2) part(warp - 2, n, d, i) = acc[n][d][i];
+        }
     }
+    __syncthreads();
+    if (warp < 2) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) part(warp, n, d, i) += acc[n][d][i];
+    }
+    __syncthreads();
+    few_finish<T, D, M, Cfg>(p, w, it, merge, row_stats, [](int, int, float) { return 1.f; });
+    __syncthreads();                                     // the results may be replaced
   }
   copy_wait<0>();
 }
 
 template <int D, int M>
-__global__ void __launch_bounds__(kFewWarps * 32, 2)
-paged_few_f32_kernel(const PagedAttnParams p, const WorkPartials w, int64_t min_weight) {
+__global__ void __launch_bounds__(kFewWarps * 32, FewCfg<float, D, M>::kBlocks)
+paged_few_f32_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w, int min_weight) {
   using T = float;
   using Cfg = FewCfg<T, D, M>;
   constexpr int E = D / 32, C = Cfg::kChunks;
@@ -453,44 +500,20 @@ paged_few_f32_kernel(const PagedAttnParams p, const WorkPartials w, int64_t min_
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) l[g] += __shfl_xor_sync(0xffffffffu, l[g], o);
 #pragma unroll
-      for (int e = 0; e < E; ++e) merge[(warp * M + g) * D + lane * E + e] = acc[g][e];
+      for (int e = 0; e < E; ++e) merge[(warp * M + g) * Cfg::kPitch + lane * E + e] = acc[g][e];
       if (lane == 0) { stat[warp * M + g] = m[g]; stat[(kFewWarps + warp) * M + g] = l[g]; }
     }
     __syncthreads();
-    const int slot = partial_slot(it);
-    for (int g = warp; g < it.rows; g += kFewWarps) {
-      float top = -INFINITY, sum = 0.f, o[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = 0.f;
+    auto factor = [&](int v, int g, float top) { return part_weight(stat[v * M + g], stat[(kFewWarps + v) * M + g], top); };
+    auto row_stats = [&](int g, float& top, float& sum) {
+      top = -INFINITY;
+      sum = 0.f;
 #pragma unroll
       for (int v = 0; v < kFewWarps; ++v) top = fmaxf(top, stat[v * M + g]);
 #pragma unroll
-      for (int v = 0; v < kFewWarps; ++v) {
-        const float mv = stat[v * M + g], lv = stat[(kFewWarps + v) * M + g];
-        const float f = mv == -INFINITY ? (isnan(lv) ? lv : 0.f) : exp2f(mv - top);
-        sum = fmaf(lv, f, sum);
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(merge[(v * M + g) * D + lane * E + e], f, o[e]);
-      }
-      if (slot >= 0) {
-        float* po = w.o + ((int64_t)slot * M + g) * D + lane * E;
-#pragma unroll
-        for (int e = 0; e < E; ++e) po[e] = o[e];
-        if (lane == 0) *reinterpret_cast<float2*>(w.ml + ((int64_t)slot * M + g) * 2) = make_float2(top, sum);
-        continue;
-      }
-      row_of<M>(p, it, g, tok, head);
-      bool nan = false;
-#pragma unroll
-      for (int e = 0; e < E; ++e) { o[e] = sum == 0.f ? 0.f : o[e] / sum; nan |= isnan(o[e]); }
-      if (__any_sync(0xffffffffu, nan)) {
-        paged_row_plain<T, D>(p, it.x, it.r, tok, head);
-        continue;
-      }
-      float* op = (float*)p.o + (int64_t)(it.x.q0 + tok) * p.so.s + (int64_t)head * p.so.h + lane * E;
-#pragma unroll
-      for (int e = 0; e < E; ++e) op[e] = o[e];
-    }
+      for (int v = 0; v < kFewWarps; ++v) sum = fmaf(stat[(kFewWarps + v) * M + g], factor(v, g, top), sum);
+    };
+    few_finish<T, D, M, Cfg>(p, w, it, merge, row_stats, factor);
     __syncthreads();                                 // queries, sums and results may be replaced
   }
   copy_wait<0>();
@@ -499,30 +522,35 @@ paged_few_f32_kernel(const PagedAttnParams p, const WorkPartials w, int64_t min_
 template <typename T, int D, int M>
 static int launch_few(const PagedAttnParams& p, cudaStream_t st) {
   using Cfg = FewCfg<T, D, M>;
-  static_assert(2 * (Cfg::kSmem + 1024 + 320) <= 233472, "two blocks per SM (1 KB each is reserved; 320 bytes of static shared memory)");
-  auto kern = [] { if constexpr (Cfg::kHalf) return paged_few_half_kernel<T, D>; else return paged_few_f32_kernel<D, M>; }();
+  auto kern = [] { if constexpr (Cfg::kHalf) return paged_few_half_kernel<T, D, M>; else return paged_few_f32_kernel<D, M>; }();
   MT_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
-  const int grid = 2 * sm_count();
+  const int grid = Cfg::kBlocks * sm_count();
   TempBuf part(partial_bytes(grid, M, D), st);
   if (!part.ok()) return MT_ERR_CUDA;
   const WorkPartials w = partials_in(part.ptr, grid, M, D);
-  kern<<<(unsigned)grid, kFewWarps * 32, Cfg::kSmem, st>>>(p, w, (int64_t)2 * Cfg::KT + kItemKeys);
+  kern<<<(unsigned)grid, kFewWarps * 32, Cfg::kSmem, st>>>(p, w, 2 * Cfg::KT + kItemKeys);
   MT_LAUNCH_CHECK();
   return launch_join<T, D, M, Cfg::KT>(p, w, grid, st);
 }
 
-template <int D>
-static int launch_few_f32(const PagedAttnParams& p, int64_t rows, cudaStream_t st) {
-  if (rows <= 1) return launch_few<float, D, 1>(p, st);
-  if (rows <= 2) return launch_few<float, D, 2>(p, st);
-  if (rows <= 4) return launch_few<float, D, 4>(p, st);
-  return launch_few<float, D, 8>(p, st);
+template <typename T, int D>
+static int launch_few_rows(const PagedAttnParams& p, int64_t rows, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (rows <= 8) return launch_few<T, D, 8>(p, st);
+    if (rows <= 16) return launch_few<T, D, 16>(p, st);
+    if (rows <= 24) return launch_few<T, D, 24>(p, st);
+    return launch_few<T, D, 32>(p, st);
+  } else {
+    if (rows <= 1) return launch_few<T, D, 1>(p, st);
+    if (rows <= 2) return launch_few<T, D, 2>(p, st);
+    if (rows <= 4) return launch_few<T, D, 4>(p, st);
+    return launch_few<T, D, 8>(p, st);
+  }
 }
 
 int attn_paged_few(const PagedAttnParams& p, int64_t row_hint, int head_dim, int dtype, cudaStream_t st) {
-  if (dtype == MT_F32) return head_dim == 64 ? launch_few_f32<64>(p, row_hint, st) : launch_few_f32<128>(p, row_hint, st);
-  if (dtype == MT_F16) return head_dim == 64 ? launch_few<__half, 64, 16>(p, st) : launch_few<__half, 128, 16>(p, st);
-  return head_dim == 64 ? launch_few<__nv_bfloat16, 64, 16>(p, st) : launch_few<__nv_bfloat16, 128, 16>(p, st);
+  MT_DISPATCH_FLOAT(dtype, T, return head_dim == 64 ? (launch_few_rows<T, 64>(p, row_hint, st)) : (launch_few_rows<T, 128>(p, row_hint, st)));
+  return MT_OK;
 }
 
 }  // namespace mt

@@ -60,7 +60,7 @@ __device__ __forceinline__ void pt_copy16(uint32_t dst, const void* src, int byt
 
 template <int D, typename T>
 __global__ void __launch_bounds__(kPtThreads, 1)
-paged_tc_kernel(const PagedAttnParams p, const WorkPartials w, int64_t min_weight, int is_bf16, int q_vec, int o_vec) {
+paged_tc_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w, int min_weight, int is_bf16, int q_vec, int o_vec) {
   using Cfg = PtCfg<D>;
   constexpr int kRing = Cfg::kRing;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -451,7 +451,7 @@ static int launch_paged_tc(const PagedAttnParams& p, cudaStream_t st) {
   if (!part.ok()) return MT_ERR_CUDA;
   const WorkPartials w = partials_in(part.ptr, grid, kPtM, D);
   auto vec = [](const void* x, mt_strides3 s) { return aligned16(x) && s.h % 8 == 0 && s.s % 8 == 0; };
-  kern<<<(unsigned)grid, kPtThreads, Cfg::kSmem, st>>>(p, w, (int64_t)2 * kPtKT + kItemKeys, std::is_same<T, __nv_bfloat16>::value,
+  kern<<<(unsigned)grid, kPtThreads, Cfg::kSmem, st>>>(p, w, 2 * kPtKT + kItemKeys, std::is_same<T, __nv_bfloat16>::value,
                                                      vec(p.q, p.sq), vec(p.o, p.so));
   MT_LAUNCH_CHECK();
   return launch_join<T, D, kPtM, kPtKT>(p, w, grid, st);

@@ -26,6 +26,7 @@ struct PagedAttnParams {
   int requests, width, rows, heads, kv_heads, group, n_pages;
   FastDiv page, by_group;
   float scale_log2;
+  int q_pairs, o_quads;                  // rows of q on 4-byte, rows of o on 8-byte (16-byte in fp32) boundaries
   int* flag;
 };
 

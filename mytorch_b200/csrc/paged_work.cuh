@@ -12,7 +12,7 @@ namespace mt {
 
 constexpr int kItemKeys = 64;            // an item's fixed cost (queries in, output out), in keys
 
-struct WorkPos { int r, hk, t, kt; };    // a key tile of an item; kt > 0: a cut inside the item
+struct alignas(16) WorkPos { int r, hk, t, kt; };    // a key tile of an item; kt > 0: a cut inside the item
 
 __device__ __forceinline__ bool same_item(const WorkPos& a, const WorkPos& b) { return a.r == b.r && a.hk == b.hk && a.t == b.t; }
 
@@ -34,7 +34,7 @@ __device__ __forceinline__ int64_t weight_upto(const PagedAttnParams& p, const P
   if (T == 0) return 0;
   const int64_t base = max(x.past, 0) + kItemKeys;
   const int64_t n = T < nt ? T : nt - 1;
-  const int64_t w = n * base + (int64_t)M * n * (n + 1) / 2 / p.group;
+  const int64_t w = n == 0 ? 0 : n * base + (int64_t)M * n * (n + 1) / 2 / p.group;
   return T < nt ? w : w + base + x.n_new;
 }
 
@@ -58,24 +58,28 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t& t
   return s - v + before;
 }
 
-struct WorkShare { WorkPos begin, end; int blocks; };    // blocks that have work
+struct WorkShare { WorkPos begin; const WorkPos* end; int blocks; };    // blocks that have work
 
-// This block's share; every thread calls it and gets the same answer. `min_weight`: at least so much per block.
+// This block's share (valid until the block ends: `end` is in shared memory); every thread calls it and gets the same answer. `min_weight`: at least so much per block.
 template <int M, int KT>
-__device__ __forceinline__ WorkShare find_share(const PagedAttnParams& p, int64_t min_weight) {
+__device__ __forceinline__ WorkShare find_share(const PagedAttnParams& p, int min_weight) {
   __shared__ int64_t sums[33];
   __shared__ WorkPos found[2];
   const int per = (p.requests + (int)blockDim.x - 1) / (int)blockDim.x;
   const int r0 = min(p.requests, (int)threadIdx.x * per), r1 = min(p.requests, r0 + per);
   auto weight = [&](const PagedRequest& x) { const int nt = row_tiles<M>(p, x); return weight_upto<M>(p, x, nt, nt) * p.kv_heads; };
   int64_t mine = 0, total;
-  for (int r = r0; r < r1; ++r) mine += weight(paged_request(p, r));
+  PagedRequest x0{};                                 // the thread's first request: the only one but for long lists
+  for (int r = r0; r < r1; ++r) {
+    const PagedRequest x = paged_request(p, r);
+    if (r == r0) x0 = x;
+    mine += weight(x);
+  }
   if (threadIdx.x < 2) found[threadIdx.x] = WorkPos{p.requests, 0, 0, 0};
   int64_t at = block_scan(mine, sums, total);
-  const int64_t many = total / min_weight;
-  const int blocks = (int)max((int64_t)1, min((int64_t)gridDim.x, many));
-  const int64_t share = total / blocks;
-  const int snap = (int)min((int64_t)INT32_MAX / 2, share / 8 / KT);    // cuts this near to an item's ends move there
+  // (every block computes the same numbers, so their rounding does not matter)
+  const int blocks = (int)fmaxf(1.f, fminf((float)gridDim.x, (float)total / (float)min_weight));
+  const int snap = (int)fminf(1e9f, (float)total / (float)blocks / (8.f * KT));    // cuts this near to an item's ends move there
   for (int e = 0; e < 2; ++e) {
     const int c = (int)blockIdx.x + e;
     if (c >= blocks) continue;                       // the list's end
@@ -83,15 +87,17 @@ __device__ __forceinline__ WorkShare find_share(const PagedAttnParams& p, int64_
     if (cut < at || cut >= at + mine) continue;
     cut -= at;
     for (int r = r0; r < r1; ++r) {
-      const PagedRequest x = paged_request(p, r);
+      const PagedRequest x = r == r0 ? x0 : paged_request(p, r);
       const int64_t w = weight(x);
       if (cut >= w) { cut -= w; continue; }
       const int nt = row_tiles<M>(p, x);
       const int64_t head = weight_upto<M>(p, x, nt, nt);
       WorkPos f;
       f.r = r;
-      f.hk = (int)(cut / head);
+      f.hk = (int)((float)cut / (float)head);
       cut -= f.hk * head;
+      for (; cut < 0; cut += head) --f.hk;
+      for (; cut >= head; cut -= head) ++f.hk;
       int lo = 0, hi = nt;                           // the last tile that begins at or before the cut
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -108,12 +114,7 @@ __device__ __forceinline__ WorkShare find_share(const PagedAttnParams& p, int64_
     }
   }
   __syncthreads();
-  WorkShare s;
-  s.begin = found[0];
-  s.end = found[1];
-  s.blocks = blocks;
-  if ((int)blockIdx.x >= blocks) s.begin = s.end;
-  return s;
+  return WorkShare{found[0], &found[1], blocks};     // without a share both are the list's end
 }
 
 struct WorkItem {
@@ -127,11 +128,13 @@ struct WorkItem {
 // Walks a share item by item.
 template <int M, int KT>
 struct WorkIter {
-  WorkPos cur, end;
+  WorkPos cur;
+  const WorkPos* last;
   int loaded, nt;
   PagedRequest x;
-  __device__ __forceinline__ void start(const WorkShare& s) { cur = s.begin; end = s.end; loaded = -1; nt = 0; }
+  __device__ __forceinline__ void start(const WorkShare& s) { cur = s.begin; last = s.end; loaded = -1; nt = 0; }
   __device__ __forceinline__ bool next(const PagedAttnParams& p, WorkItem& it) {
+    const WorkPos end = *last;
     for (;;) {
       if (cur.r >= p.requests) return false;
       if (cur.r > end.r || (cur.r == end.r && (cur.hk > end.hk || (cur.hk == end.hk && (cur.t > end.t || (cur.t == end.t && cur.kt >= end.kt))))))
@@ -197,6 +200,21 @@ __device__ __forceinline__ void row_of(const PagedAttnParams& p, const WorkItem&
   head = it.hk * p.group + (int)(at - (uint32_t)token * p.group);
 }
 
+// Lane l's D/32 neighbouring elements of an output row.
+template <typename T, int E>
+__device__ __forceinline__ void store_row(const PagedAttnParams& p, const PagedRequest& x, int token, int head, const float (&v)[E]) {
+  T* op = (T*)p.o + (int64_t)(x.q0 + token) * p.so.s + (int64_t)head * p.so.h + (threadIdx.x & 31) * E;
+  if (p.o_quads) {
+    struct alignas(sizeof(T) * E) Pack { T t[E]; } pack;
+#pragma unroll
+    for (int e = 0; e < E; ++e) pack.t[e] = from_f<T>(v[e]);
+    *reinterpret_cast<Pack*>(op) = pack;
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) op[e] = from_f<T>(v[e]);
+  }
+}
+
 // One output row (a token's head) by one warp, straight from the definition: lane l holds D/32
 // neighbouring elements of q and o, scores are fp32 dot products, and only the visible keys are touched.
 // The tiled kernels' masks are weights of zero, which a value that is not finite turns into NaN; rows
@@ -229,70 +247,73 @@ __device__ __noinline__ void paged_row_plain(const PagedAttnParams& p, PagedRequ
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = fmaf(w, to_f(vp[at + e]), o[e] * c);
   }
-  T* op = (T*)p.o + (int64_t)(x.q0 + i) * p.so.s + (int64_t)h * p.so.h + lane * E;
 #pragma unroll
-  for (int e = 0; e < E; ++e) op[e] = from_f<T>(l == 0.f ? 0.f : o[e] / l);
+  for (int e = 0; e < E; ++e) o[e] = l == 0.f ? 0.f : o[e] / l;
+  store_row<T, E>(p, x, i, h, o);
 }
 
 // Joins the partial results of the items that cuts run through: block (c, y) takes the item whose first cut
-// is the one between blocks c - 1 and c, a warp one row at a time. The pieces are weighted in the order of
-// the keys.
+// is the one between blocks c and c + 1, a warp one row at a time. A lane looks one piece up, so that a row of up to
+// 32 pieces costs four round trips to L2 whatever their number (8 us for seven pieces looked up one after the other,
+// 2.5 so); the pieces are added in the order of the keys.
 template <typename T, int D, int M, int KT>
 __global__ void __launch_bounds__(128)
-paged_join_kernel(const PagedAttnParams p, const WorkPartials w, int grid) {
+paged_join_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w, int grid) {
   constexpr int E = D / 32;
   grid_dependency_wait();
   const int blocks = w.cuts[grid].r, c = (int)blockIdx.x + 1;
-  if (c >= blocks) return;
   const WorkPos cut = w.cuts[c], before = w.cuts[c - 1];
-  if (cut.kt == 0 || (before.kt > 0 && same_item(before, cut))) return;
-  int last = c;                                      // the item's pieces: slot 2c-1, then 2j of blocks c..last
-  while (last + 1 < blocks && same_item(w.cuts[last + 1], cut) && w.cuts[last + 1].kt > 0) ++last;
-  const int pieces = last - c + 2;
+  if (c >= blocks || cut.kt == 0 || (before.kt > 0 && same_item(before, cut))) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   WorkItem it;
   it.r = cut.r; it.hk = cut.hk; it.t = cut.t;
   it.x = paged_request(p, cut.r);
   it.rows = (int)min((int64_t)M, (int64_t)it.x.n_new * p.group - (int64_t)cut.t * M);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // an empty piece (two cuts at one key tile) was not written
-  auto slot_of = [&](int i) {
-    if (i == 0) return 2 * (c - 1) + 1;
-    const int j = c + i - 1;
-    return j < last && w.cuts[j + 1].kt == w.cuts[j].kt ? -1 : 2 * j;
-  };
+  int last = c;                                      // the item's pieces: slot 2c-1, then slots 2j of blocks c..last
+  for (;;) {
+    const int j = last + 1 + lane;
+    const bool inside = j < blocks && same_item(w.cuts[j], cut) && w.cuts[j].kt > 0;
+    const uint32_t out = __ballot_sync(0xffffffffu, !inside);
+    if (out) { last += __ffs((int)out) - 1; break; }
+    last += 32;
+  }
+  const int pieces = last - c + 2;
   for (int row = (int)blockIdx.y * 4 + warp; row < it.rows; row += 4 * gridDim.y) {
-    float m = -INFINITY;
-    for (int i = lane; i < pieces; i += 32) {
-      const int s = slot_of(i);
-      if (s >= 0) m = fmaxf(m, w.ml[((int64_t)s * M + row) * 2]);
-    }
-    m = warp_max(m);
-    float l = 0.f, o[E];
+    float m = -INFINITY, l = 0.f, o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < pieces; ++i) {
-      const int s = slot_of(i);
-      if (s < 0) continue;
-      const float* ml = w.ml + ((int64_t)s * M + row) * 2;
-      const float a = ml[0] == -INFINITY ? (isnan(ml[1]) ? ml[1] : 0.f) : exp2f(ml[0] - m);
-      l = fmaf(ml[1], a, l);
-      const float* src = w.o + ((int64_t)s * M + row) * D + lane * E;
+    for (int i0 = 0; i0 < pieces; i0 += 32) {
+      const int i = i0 + lane, j = c + i - 1;
+      int slot = i < pieces ? (i == 0 ? 2 * c - 1 : 2 * j) : -1;
+      if (slot >= 0 && i > 0 && j < last && w.cuts[j + 1].kt == w.cuts[j].kt) slot = -1;   // two cuts at one key tile: nothing was written
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (slot >= 0) ml = *reinterpret_cast<const float2*>(w.ml + ((int64_t)slot * M + row) * 2);
+      const float mn = fmaxf(m, warp_max(ml.x));
+      // without a maximum there are no weights, or only NaN ones, which stay
+      const float keep = m == -INFINITY ? 0.f : exp2f(m - mn), a = ml.x == -INFINITY ? (isnan(ml.y) ? ml.y : 0.f) : exp2f(ml.x - mn);
+      m = mn;
+      l = l * keep + warp_sum(ml.y * a);
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = fmaf(src[e], a, o[e]);
+      for (int e = 0; e < E; ++e) o[e] *= keep;
+      const int n = min(32, pieces - i0);
+#pragma unroll 8
+      for (int k = 0; k < n; ++k) {
+        const int s = __shfl_sync(0xffffffffu, slot, k);
+        const float f = __shfl_sync(0xffffffffu, a, k);
+        struct alignas(4 * E) Pack { float t[E]; } v{};
+        if (s >= 0) v = *reinterpret_cast<const Pack*>(w.o + ((int64_t)s * M + row) * D + lane * E);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(v.t[e], f, o[e]);
+      }
     }
     int token, head;
     row_of<M>(p, it, row, token, head);
     bool nan = false;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-    for (int e = 0; e < E; ++e) { o[e] = l == 0.f ? 0.f : o[e] / l; nan |= isnan(o[e]); }
-    if (__any_sync(0xffffffffu, nan)) {
-      paged_row_plain<T, D>(p, it.x, it.r, token, head);
-      continue;
-    }
-    T* op = (T*)p.o + (int64_t)(it.x.q0 + token) * p.so.s + (int64_t)head * p.so.h + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) op[e] = from_f<T>(o[e]);
+    for (int e = 0; e < E; ++e) { o[e] *= inv; nan |= isnan(o[e]); }
+    if (__any_sync(0xffffffffu, nan)) paged_row_plain<T, D>(p, it.x, it.r, token, head);
+    else store_row<T, E>(p, it.x, token, head, o);
   }
 }
 
