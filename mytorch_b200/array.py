@@ -75,8 +75,8 @@ class DeviceArray:
 
     def __init__(self, ptr, shape, dtype, base=None, owns=False):
         self.ptr = int(ptr)
-        self.shape = tuple(int(s) for s in shape)
-        self.dtype = norm_dtype(dtype)
+        self.shape = tuple(map(int, shape))
+        self.dtype = dtype if dtype in _DT else norm_dtype(dtype)
         self._base = base
         self._owns = owns
 
@@ -147,7 +147,8 @@ class DeviceArray:
 
     @property
     def code(self):
-        return code(self.dtype)
+        c = _DT[self.dtype][0]
+        return code(self.dtype) if c is None else c
 
     @property
     def __cuda_array_interface__(self):

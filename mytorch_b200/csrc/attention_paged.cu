@@ -44,7 +44,7 @@ int mt_attn_paged(const void* q, const void* k_pages, const void* v_pages, void*
   MT_REQUIRE(head_dim == 64 || head_dim == 128, "attn_paged: head_dim must be 64 or 128");
   MT_REQUIRE(width >= 1 && width < (1ll << 31) && page_size >= 1 && page_size < (1ll << 30) && width * page_size < (1ll << 31) && n_pages >= 0 &&
              n_pages < (1ll << 31), "attn_paged: a table row has to span between 1 and 2^31 - 1 positions");
-  MT_REQUIRE(requests <= (1 << 20) && rows * heads < (1ll << 31) && max_new >= 0, "attn_paged: too many query rows");
+  MT_REQUIRE(requests <= (1 << 20) && rows < (1ll << 28) && heads < (1ll << 28) && rows * heads < (1ll << 28) && max_new >= 0, "attn_paged: too many query rows");
   const int64_t unit = 16 / (int64_t)dtype_size(dtype);
   MT_REQUIRE(spages.b % unit == 0 && spages.h % unit == 0 && spages.s % unit == 0 && aligned16(k_pages) && aligned16(v_pages),
              "attn_paged: the rows of the pools must be 16-byte aligned");

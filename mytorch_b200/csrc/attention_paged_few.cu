@@ -79,47 +79,53 @@ template <typename T> __device__ __forceinline__ uint32_t pair_bits(T a, T b) {
   return (uint32_t)*reinterpret_cast<uint16_t*>(&a) | (uint32_t)*reinterpret_cast<uint16_t*>(&b) << 16;
 }
 
-// A warp's ring of key and value tiles: the load side of the pipeline.
+// A warp's ring of key and value tiles: the load side of the pipeline. The warp holds 32 neighbouring entries of the
+// request's table, one per lane; a new window is asked for when the next tile is not in it, while the
+// tile before is on its way.
 template <typename T, int D, int M>
 struct FewLoader {
   using Cfg = FewCfg<T, D, M>;
   WorkIter<M, Cfg::KT> iter;
   WorkItem it;
   bool valid;
-  int kt, page;
+  int kt, window, page;                  // window: first table entry held, -1: none; page: lane's entry
   uint32_t ring;
   uint32_t* masks;                       // [stages]: which of the tile's rows are there
 
+  __device__ __forceinline__ int first_key(int warp) const { return kt * Cfg::KT + warp * Cfg::kRows; }
   __device__ __forceinline__ void advance(const PagedAttnParams& p, int warp, int lane) {
     while (valid && kt >= it.k1) {
       valid = iter.next(p, it);
-      if (valid) kt = it.k0;
+      if (valid) { kt = it.k0; window = -1; }
     }
-    page = -1;
-    if (valid) {
-      const int key = kt * Cfg::KT + warp * Cfg::kRows + (lane % Cfg::kRows);
-      if (key < it.keys) {
-        page = p.tables[(int64_t)it.r * p.width + p.page.div((uint32_t)key)];
-        if ((unsigned)page >= (unsigned)p.n_pages) {
-          if (p.flag) atomicMax(p.flag, kPagedFlag);
-          page = -1;
-        }
-      }
-    }
+    if (!valid) return;
+    const int key0 = first_key(warp), key1 = min(key0 + Cfg::kRows, it.keys) - 1;
+    if (key1 < key0) return;                                     // no row of this warp's in the tile
+    const int a = (int)p.page.div((uint32_t)key0), b = (int)p.page.div((uint32_t)key1);
+    if (window >= 0 && b < window + 32) return;
+    window = a;
+    page = a + lane < p.width ? p.tables[(int64_t)it.r * p.width + a + lane] : -1;
   }
   __device__ __forceinline__ void start(const PagedAttnParams& p, const WorkShare& s, int warp, int lane) {
     iter.start(s);
     it.k1 = 0;
     kt = 0;
+    window = -1;
     valid = true;
     advance(p, warp, lane);
   }
   // Queues the loads of the tile under the cursor into `stage`, one commit group per call.
   __device__ __forceinline__ void issue(const PagedAttnParams& p, int stage, int warp, int lane) {
     if (valid) {
-      const int key = kt * Cfg::KT + warp * Cfg::kRows + (lane % Cfg::kRows);
-      const uint32_t in_page = (uint32_t)key - p.page.div((uint32_t)key) * p.page.d;
-      const int64_t off = page >= 0 ? (int64_t)page * p.sc.b + (int64_t)in_page * p.sc.s + (int64_t)it.hk * p.sc.h : -1;
+      const int key = first_key(warp) + (lane % Cfg::kRows);
+      const uint32_t at = p.page.div((uint32_t)key);
+      const int id = __shfl_sync(0xffffffffu, page, (int)at - window);       // lanes behind the last key read anything
+      int64_t off = -1;
+      if (key < it.keys) {
+        if ((unsigned)id < (unsigned)p.n_pages)
+          off = (int64_t)id * p.sc.b + (int64_t)(key - (int)(at * p.page.d)) * p.sc.s + (int64_t)it.hk * p.sc.h;
+        else if (p.flag) atomicMax(p.flag, kPagedFlag);
+      }
       const uint32_t mask = __ballot_sync(0xffffffffu, off >= 0) & (uint32_t)((1ull << Cfg::kRows) - 1);
       if (lane == 0) masks[stage] = mask;
       if (mask) {
@@ -186,7 +192,7 @@ __device__ __forceinline__ float part_weight(float m, float l, float top) {
 
 template <typename T, int D, int M>
 __global__ void __launch_bounds__(kFewWarps * 32, FewCfg<T, D, M>::kBlocks)
-paged_few_half_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w, int min_weight) {
+paged_few_half_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w, int least, uint32_t slope) {
   using Cfg = FewCfg<T, D, M>;
   constexpr int NT = M / 8, KM = Cfg::kRows / 16, C = Cfg::kChunks;
   extern __shared__ __align__(128) uint8_t few_smem[];
@@ -194,8 +200,9 @@ paged_few_half_kernel(const __grid_constant__ PagedAttnParams p, const WorkParti
   float* stat = reinterpret_cast<float*>(few_smem + Cfg::kOffStat);            // [warps][M] maxima, then sums
   uint32_t* masks = reinterpret_cast<uint32_t*>(stat + kFewWarps * M * 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  grid_dependency_wait();
   allow_dependents();
-  const WorkShare share = find_share<M, Cfg::KT>(p, min_weight);
+  const WorkShare share = find_share<M, Cfg::KT>(p, least, slope);
   publish_share(share, w);
   FewLoader<T, D, M> load;
   load.ring = smem_addr(few_smem) + warp * Cfg::kRing;
@@ -393,7 +400,7 @@ paged_few_half_kernel(const __grid_constant__ PagedAttnParams p, const WorkParti
 
 template <int D, int M>
 __global__ void __launch_bounds__(kFewWarps * 32, FewCfg<float, D, M>::kBlocks)
-paged_few_f32_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w, int min_weight) {
+paged_few_f32_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w, int least, uint32_t slope) {
   using T = float;
   using Cfg = FewCfg<T, D, M>;
   constexpr int E = D / 32, C = Cfg::kChunks;
@@ -403,8 +410,9 @@ paged_few_f32_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartia
   float* stat = reinterpret_cast<float*>(few_smem + Cfg::kOffStat);
   uint32_t* masks = reinterpret_cast<uint32_t*>(stat + kFewWarps * M * 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  grid_dependency_wait();
   allow_dependents();
-  const WorkShare share = find_share<M, Cfg::KT>(p, min_weight);
+  const WorkShare share = find_share<M, Cfg::KT>(p, least, slope);
   publish_share(share, w);
   FewLoader<T, D, M> load;
   load.ring = smem_addr(few_smem) + warp * Cfg::kRing;
@@ -523,13 +531,14 @@ template <typename T, int D, int M>
 static int launch_few(const PagedAttnParams& p, cudaStream_t st) {
   using Cfg = FewCfg<T, D, M>;
   auto kern = [] { if constexpr (Cfg::kHalf) return paged_few_half_kernel<T, D, M>; else return paged_few_f32_kernel<D, M>; }();
-  MT_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
+  static SmemLimit limit;
+  if (int rc = limit.raise((const void*)kern, Cfg::kSmem)) return rc;
   const int grid = Cfg::kBlocks * sm_count();
   TempBuf part(partial_bytes(grid, M, D), st);
   if (!part.ok()) return MT_ERR_CUDA;
   const WorkPartials w = partials_in(part.ptr, grid, M, D);
-  kern<<<(unsigned)grid, kFewWarps * 32, Cfg::kSmem, st>>>(p, w, 2 * Cfg::KT + kItemKeys);
-  MT_LAUNCH_CHECK();
+  MT_CHECK_CUDA(launch_overlapped(kern, dim3((unsigned)grid), dim3(kFewWarps * 32), Cfg::kSmem, st, p, w, 3, tile_slope<M, Cfg::KT>(p.group)));
+  count_launch();
   return launch_join<T, D, M, Cfg::KT>(p, w, grid, st);
 }
 

@@ -60,7 +60,7 @@ __device__ __forceinline__ void pt_copy16(uint32_t dst, const void* src, int byt
 
 template <int D, typename T>
 __global__ void __launch_bounds__(kPtThreads, 1)
-paged_tc_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w, int min_weight, int is_bf16, int q_vec, int o_vec) {
+paged_tc_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w, int least, uint32_t slope, int is_bf16, int q_vec, int o_vec) {
   using Cfg = PtCfg<D>;
   constexpr int kRing = Cfg::kRing;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -89,8 +89,9 @@ paged_tc_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w,
     tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
   }
+  grid_dependency_wait();
   allow_dependents();
-  const WorkShare share = find_share<kPtM, kPtKT>(p, min_weight);
+  const WorkShare share = find_share<kPtM, kPtKT>(p, least, slope);
   publish_share(share, w);
   tc_fence_before();
   __syncthreads();
@@ -445,15 +446,16 @@ template <int D, typename T>
 static int launch_paged_tc(const PagedAttnParams& p, cudaStream_t st) {
   using Cfg = PtCfg<D>;
   auto kern = paged_tc_kernel<D, T>;
-  MT_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
+  static SmemLimit limit;
+  if (int rc = limit.raise((const void*)kern, Cfg::kSmem)) return rc;
   const int grid = sm_count();
   TempBuf part(partial_bytes(grid, kPtM, D), st);
   if (!part.ok()) return MT_ERR_CUDA;
   const WorkPartials w = partials_in(part.ptr, grid, kPtM, D);
   auto vec = [](const void* x, mt_strides3 s) { return aligned16(x) && s.h % 8 == 0 && s.s % 8 == 0; };
-  kern<<<(unsigned)grid, kPtThreads, Cfg::kSmem, st>>>(p, w, 2 * kPtKT + kItemKeys, std::is_same<T, __nv_bfloat16>::value,
-                                                     vec(p.q, p.sq), vec(p.o, p.so));
-  MT_LAUNCH_CHECK();
+  MT_CHECK_CUDA(launch_overlapped(kern, dim3((unsigned)grid), dim3(kPtThreads), Cfg::kSmem, st, p, w, 3, tile_slope<kPtM, kPtKT>(p.group),
+                                  std::is_same<T, __nv_bfloat16>::value, vec(p.q, p.sq), vec(p.o, p.so)));
+  count_launch();
   return launch_join<T, D, kPtM, kPtKT>(p, w, grid, st);
 }
 

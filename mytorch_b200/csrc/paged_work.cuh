@@ -7,10 +7,9 @@
 // and sum per row) that a second kernel joins in the order of the keys, so results do not depend on timing.
 #pragma once
 #include "paged.cuh"
+#include <atomic>
 
 namespace mt {
-
-constexpr int kItemKeys = 64;            // an item's fixed cost (queries in, output out), in keys
 
 struct alignas(16) WorkPos { int r, hk, t, kt; };    // a key tile of an item; kt > 0: a cut inside the item
 
@@ -28,14 +27,15 @@ __device__ __forceinline__ int tile_keys(const PagedAttnParams& p, const PagedRe
   return visible_keys(x, (int)p.by_group.div((uint32_t)(rows - 1)));
 }
 
-// Weight of the first T of nt tiles of one head: closed form, increasing.
-template <int M>
-__device__ __forceinline__ int64_t weight_upto(const PagedAttnParams& p, const PagedRequest& x, int T, int nt) {
-  if (T == 0) return 0;
-  const int64_t base = max(x.past, 0) + kItemKeys;
-  const int64_t n = T < nt ? T : nt - 1;
-  const int64_t w = n == 0 ? 0 : n * base + (int64_t)M * n * (n + 1) / 2 / p.group;
-  return T < nt ? w : w + base + x.n_new;
+// Weight of the first T of nt tiles of one head, in key tiles: increasing, in closed form and free of
+// divisions (a block's first 2 us are this arithmetic, and every block does it). A tile's weight is one for
+// its fixed cost (queries in, output out) and the keys that its rows see; `slope` is what a tile sees more than the one before, M / (group * KT), in
+// units of 2^-16.
+template <int KT>
+__device__ __forceinline__ int64_t weight_upto(const PagedRequest& x, uint32_t slope, int T, int nt) {
+  const int base = max(x.past, 0) / KT + 1, n = min(T, nt - 1);
+  const int64_t w = (int64_t)n * base + (int64_t)(((uint64_t)((int64_t)n * (n + 1)) >> 1) * slope >> 16);
+  return T < nt || nt == 0 ? w : w + base + x.n_new / KT;
 }
 
 // Exclusive prefix sum of one value per thread and the block's total. `sh`: 33 values.
@@ -60,62 +60,73 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t& t
 
 struct WorkShare { WorkPos begin; const WorkPos* end; int blocks; };    // blocks that have work
 
-// This block's share (valid until the block ends: `end` is in shared memory); every thread calls it and gets the same answer. `min_weight`: at least so much per block.
+// This block's share (valid until the block ends: `end` is in shared memory); every thread calls it and gets
+// the same answer. `least`: at least so many key tiles per block, fixed costs included. Threads sum up the
+// weights of their requests; then warp 0 finds where the share begins and warp 1 where it ends.
 template <int M, int KT>
-__device__ __forceinline__ WorkShare find_share(const PagedAttnParams& p, int min_weight) {
+__device__ __forceinline__ WorkShare find_share(const PagedAttnParams& p, int least, uint32_t slope) {
   __shared__ int64_t sums[33];
+  __shared__ int64_t before[2];          // of the two cuts: weights before the thread's requests
+  __shared__ int owner[2];
   __shared__ WorkPos found[2];
   const int per = (p.requests + (int)blockDim.x - 1) / (int)blockDim.x;
   const int r0 = min(p.requests, (int)threadIdx.x * per), r1 = min(p.requests, r0 + per);
-  auto weight = [&](const PagedRequest& x) { const int nt = row_tiles<M>(p, x); return weight_upto<M>(p, x, nt, nt) * p.kv_heads; };
   int64_t mine = 0, total;
-  PagedRequest x0{};                                 // the thread's first request: the only one but for long lists
   for (int r = r0; r < r1; ++r) {
     const PagedRequest x = paged_request(p, r);
-    if (r == r0) x0 = x;
-    mine += weight(x);
+    const int nt = row_tiles<M>(p, x);
+    mine += weight_upto<KT>(x, slope, nt, nt) * p.kv_heads;
   }
-  if (threadIdx.x < 2) found[threadIdx.x] = WorkPos{p.requests, 0, 0, 0};
-  int64_t at = block_scan(mine, sums, total);
-  // (every block computes the same numbers, so their rounding does not matter)
-  const int blocks = (int)fmaxf(1.f, fminf((float)gridDim.x, (float)total / (float)min_weight));
-  const int snap = (int)fminf(1e9f, (float)total / (float)blocks / (8.f * KT));    // cuts this near to an item's ends move there
+  if (threadIdx.x < 2) owner[threadIdx.x] = -1;
+  const int64_t at = block_scan(mine, sums, total);
+  // Every block computes the same numbers, and rounding keeps the order of the cuts: that is all they need.
+  const int blocks = (int)fmaxf(1.f, fminf((float)gridDim.x, (float)total / (float)least));
+  const int snap = (int)fminf(1e9f, (float)total / (float)(8 * blocks));    // cuts this near to an item's ends move there
+  auto cut_of = [&](int c) { return (int64_t)((float)total * ((float)c / (float)blocks)); };
+#pragma unroll
   for (int e = 0; e < 2; ++e) {
-    const int c = (int)blockIdx.x + e;
-    if (c >= blocks) continue;                       // the list's end
-    int64_t cut = (int64_t)((double)total * c / blocks);
-    if (cut < at || cut >= at + mine) continue;
-    cut -= at;
-    for (int r = r0; r < r1; ++r) {
-      const PagedRequest x = r == r0 ? x0 : paged_request(p, r);
-      const int64_t w = weight(x);
-      if (cut >= w) { cut -= w; continue; }
-      const int nt = row_tiles<M>(p, x);
-      const int64_t head = weight_upto<M>(p, x, nt, nt);
-      WorkPos f;
-      f.r = r;
-      f.hk = (int)((float)cut / (float)head);
+    const int64_t cut = cut_of((int)blockIdx.x + e);
+    if ((int)blockIdx.x + e < blocks && cut >= at && cut < at + mine) { before[e] = at; owner[e] = r0; }
+  }
+  __syncthreads();
+  const int e = threadIdx.x >> 5;
+  if (e < 2 && (threadIdx.x & 31) == 0) {
+    WorkPos f{p.requests, 0, 0, 0};                  // the list's end
+    if (owner[e] >= 0) {
+      int64_t cut = cut_of((int)blockIdx.x + e) - before[e], head = 0;
+      PagedRequest x{};
+      int nt = 0;
+      for (f.r = owner[e];; ++f.r) {
+        x = paged_request(p, f.r);
+        nt = row_tiles<M>(p, x);
+        head = weight_upto<KT>(x, slope, nt, nt);
+        if (cut < head * p.kv_heads) break;
+        cut -= head * p.kv_heads;
+      }
+      f.hk = (int)__fdividef((float)cut, (float)head);
       cut -= f.hk * head;
       for (; cut < 0; cut += head) --f.hk;
       for (; cut >= head; cut -= head) ++f.hk;
       int lo = 0, hi = nt;                           // the last tile that begins at or before the cut
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (weight_upto<M>(p, x, mid, nt) <= cut) lo = mid; else hi = mid;
+        if (weight_upto<KT>(x, slope, mid, nt) <= cut) lo = mid; else hi = mid;
       }
-      const int64_t begin = weight_upto<M>(p, x, lo, nt), width = weight_upto<M>(p, x, lo + 1, nt) - begin;
+      const int64_t begin = weight_upto<KT>(x, slope, lo, nt), width = weight_upto<KT>(x, slope, lo + 1, nt) - begin;
       const int n = (tile_keys<M>(p, x, lo) + KT - 1) / KT;
-      const int kt = (int)((double)(cut - begin) * n / width);
+      const int kt = min(n - 1, (int)((float)(cut - begin) * (float)n / (float)width));
       f.t = lo;
       f.kt = kt <= snap ? 0 : kt;
       if (f.kt && n - kt <= snap) { ++f.t; f.kt = 0; }
-      found[e] = f;
-      break;
     }
+    found[e] = f;
   }
   __syncthreads();
   return WorkShare{found[0], &found[1], blocks};     // without a share both are the list's end
 }
+
+template <int M, int KT>
+inline uint32_t tile_slope(int group) { return (uint32_t)(((uint64_t)M << 16) / ((uint64_t)group * KT)); }
 
 struct WorkItem {
   int r, hk, t;
@@ -183,6 +194,19 @@ inline WorkPartials partials_in(void* buf, int blocks, int M, int D) {
   w.cuts = (WorkPos*)(w.ml + (size_t)blocks * 2 * M * 2);
   return w;
 }
+
+// A kernel's limit on dynamic shared memory, raised once per device (racing first calls raise it twice, harmlessly).
+struct SmemLimit {
+  std::atomic<bool> done[16] = {};
+  int raise(const void* kern, int bytes) {
+    int dev = 0;
+    MT_CHECK_CUDA(cudaGetDevice(&dev));
+    if (dev >= 0 && dev < 16 && done[dev].load(std::memory_order_acquire)) return MT_OK;
+    MT_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (dev >= 0 && dev < 16) done[dev].store(true, std::memory_order_release);
+    return MT_OK;
+  }
+};
 
 // The block whose share begins at blockIdx.x tells the joining kernel so.
 __device__ __forceinline__ void publish_share(const WorkShare& s, const WorkPartials& w) {
@@ -261,6 +285,7 @@ __global__ void __launch_bounds__(128)
 paged_join_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w, int grid) {
   constexpr int E = D / 32;
   grid_dependency_wait();
+  allow_dependents();
   const int blocks = w.cuts[grid].r, c = (int)blockIdx.x + 1;
   const WorkPos cut = w.cuts[c], before = w.cuts[c - 1];
   if (c >= blocks || cut.kt == 0 || (before.kt > 0 && same_item(before, cut))) return;

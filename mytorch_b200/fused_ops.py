@@ -377,14 +377,18 @@ def fused_rope_rmsnorm_backward(dyq, dyk, yq, yk, rstd_q, rstd_k, cos, sin):
 def _ints(name, a, *shape):
     """An int32 array of the given shape (None = any extent)."""
     a = _A(a)
-    if a.dtype != "int32" or len(a.shape) != len(shape) or any(n is not None and n != m for n, m in zip(shape, a.shape)):
-        raise ValueError(f"{name}: int32 {list(shape)} expected, got {a.dtype} {list(a.shape)}")
-    return a
+    if a.dtype == "int32" and len(a.shape) == len(shape):
+        for want, got in zip(shape, a.shape):
+            if want is not None and want != got:
+                break
+        else:
+            return a
+    raise ValueError(f"{name}: int32 {list(shape)} expected, got {a.dtype} {list(a.shape)}")
 
 
 def _pools(k_pages, v_pages):
     k, v = _A(k_pages), _A(v_pages)
-    if k.ndim != 4 or k.shape != v.shape:
+    if len(k.shape) != 4 or k.shape != v.shape:
         raise ValueError(f"pools of keys and values are [pages, kv_heads, page_size, head_dim] both, got {k.shape} and {v.shape}")
     return k, v
 
@@ -431,7 +435,7 @@ def fused_paged_append(k, v, k_pages, v_pages, slot, strides=None):
     k_pages, v_pages = _pools(k_pages, v_pages)
     _check_float(k, v, k_pages, v_pages)
     P, H, S, D = k_pages.shape
-    if k.ndim != 3 or k.shape != v.shape or k.shape[1:] != (H, D):
+    if len(k.shape) != 3 or k.shape != v.shape or k.shape[1:] != (H, D):
         raise ValueError(f"new keys and values are [rows, {H}, {D}] both, got {k.shape} and {v.shape}")
     slot = _ints("slot", slot, k.shape[0])
     sk, sv = strides or (_lib.Strides3(0, D, H * D),) * 2
@@ -449,7 +453,7 @@ def fused_paged_attention(q, k_pages, v_pages, tables, starts, kv_len, max_new=N
     k_pages, v_pages = _pools(k_pages, v_pages)
     _check_float(q, k_pages, v_pages)
     P, Hk, S, D = k_pages.shape
-    if q.ndim != 3 or q.shape[2] != D or q.shape[1] % Hk:
+    if len(q.shape) != 3 or q.shape[2] != D or q.shape[1] % Hk:
         raise ValueError(f"q is [rows, heads, {D}] with a multiple of {Hk} heads, got {q.shape}")
     N, H, _ = q.shape
     kv_len = _ints("kv_len", kv_len, None)
