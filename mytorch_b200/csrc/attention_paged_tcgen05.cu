@@ -1,22 +1,25 @@
 // Attention over pages on the tensor cores, fp16/bf16: prompts, chunks of prompts and batches that mix
 // them with decoding requests.
 //
-// Persistent, one CTA per SM, 416 threads; a CTA walks its share of the work (paged_work.cuh). An item is
+// Persistent, one CTA per SM, 512 threads; a CTA walks its share of the work (paged_work.cuh). An item is
 // 256 query rows (tokens times the query heads of the group, so grouped heads fill tiles and share the loads) of one
 // key/value head, in two subtiles A and B of 128, against key tiles of 128:
-//   warps 8-11  loaders: key and value rows lie wherever their pages are, so they come by 16-byte cp.async
-//               (a thread looks up one row's page, a tile ahead, and hands the address to the lanes that copy it),
-//               written in the 128-byte swizzle that the MMA reads, into one ring in the order of use
-//               K0 K1 V0 K2 V1 ...; two groups stay in flight behind the one being queued. Rows behind the
-//               last key or on a bad page are zeros, their bits in a mask of the tile are clear.
+//   warps 8-11  loaders: key and value rows lie wherever their pages are. A tile whose 128 rows are all there
+//               comes by TMA, a box per page (pages of 8 to 128 rows that divide 128, or multiples of 128 rows; zeros for
+//               a page outside the pool); the others, and every tile of odd page sizes, by 16-byte cp.async row by row, with
+//               zeros behind the last key, in the 128-byte swizzle that the MMA reads (it takes a warp 1000 cycles
+//               to queue its 32 rows of one tile, as long as the tile's products run).
+//               One ring in the order of use, K0 K1 V0 K2 V1 ...; page lookups run a tile ahead; which of a tile's rows
+//               are there is a mask next to it.
 //   warp 12     MMA issuer: S_A = Q_A K^T and S_B = Q_B K^T into tensor memory, then per tile O_A += P_A V and the
 //               next S_A while subtile B is in its softmax, O_B += P_B V and the next S_B while A is: the
 //               tensor pipe always has the other subtile's products.
-//   warps 0-3, 4-7  softmax of A and B: a thread owns a row (TMEM lane), reads its 128 scores twice (maximum;
-//               weights) in pieces of 32, and writes the weights as packed half pairs over the scores, which
-//               nobody reads any more; P is the A operand straight from tensor memory. The running maximum
-//               only moves, and O in tensor memory is only rescaled, when it grew by more than 2^8. The
-//               weights are rounded to the type for the product (half a step, as the output is); sums are fp32.
+//   warps 0-3, 4-7  softmax of A and B: a thread owns a row (TMEM lane) and holds its 128 scores in registers (the loaders
+//               and the issuer hand registers over by setmaxnreg; in pieces of 32 scores, read twice, a tile took 4000 cycles),
+//               and writes the weights as packed half pairs over the scores; P is the A operand straight from
+//               tensor memory. The running maximum only moves, and O in tensor memory is only rescaled, when it
+//               grew by more than 2^8. The weights are rounded to the type for the product (half a step, as
+//               the output is); sums are fp32.
 // Tensor memory: S_A, S_B (128 columns each), O_A, O_B (D each).
 //
 // Roofline: tensor pipe, 4 D operations per (row, visible key), or the exponentials (16 per clock per SM,
@@ -31,17 +34,21 @@ namespace mt {
 using namespace sm100;
 
 constexpr int kPtM = 256, kPtKT = 128;
-constexpr int kPtThreads = 416;
+constexpr int kPtThreads = 512;
+// Registers per thread: 128 at launch; 2 x 128 threads of softmax take what the other 2 x 128 give back.
+constexpr int kPtRegsMore = 184, kPtRegsLess = 72;
+static_assert(kPtRegsMore + kPtRegsLess <= 2 * 128, "more registers than the block was launched with");
 constexpr int kPtAbort = 105;
 
 template <int D> struct PtCfg {
   static constexpr int kChunks = D / 64;                 // 64-column (128-byte) slices of head_dim
   static constexpr int kTile = 128 * D * 2;              // 128 rows of Q, K or V
-  static constexpr int kRing = D == 128 ? 5 : 8;
+  static constexpr int kRing = D == 128 ? 4 : 8;
   static constexpr int kOffRing = 2 * kTile;             // behind Q_A and Q_B
   static constexpr int kOffBar = kOffRing + kRing * kTile;
   static constexpr int kOffMask = kOffBar + 256;         // [16 tiles][4 words]
-  static constexpr int kSmem = kOffMask + 256;
+  static constexpr int kOffStage = kOffMask + 768;       // a softmax warp's 32 rows x 128 bytes on their way out, swizzled
+  static constexpr int kSmem = kOffStage + 8 * 4096;
   static constexpr int kColO = 256;
   static_assert(kSmem + 1024 <= 232448, "shared memory of one CTA, static part included");
 };
@@ -60,7 +67,9 @@ __device__ __forceinline__ void pt_copy16(uint32_t dst, const void* src, int byt
 
 template <int D, typename T>
 __global__ void __launch_bounds__(kPtThreads, 1)
-paged_tc_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w, int least, uint32_t slope, int is_bf16, int q_vec, int o_vec) {
+paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                const __grid_constant__ PagedAttnParams p, const WorkPartials w, int least, uint32_t slope, int is_bf16, int q_vec,
+                int o_vec, int box_rows) {
   using Cfg = PtCfg<D>;
   constexpr int kRing = Cfg::kRing;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -101,7 +110,9 @@ paged_tc_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w,
   iter.start(share);
   WorkItem it;
 
-  if (warp >= 8 && warp < 12) {
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPtRegsLess));
+  if (warp < 12) {
     // ------------------------------------------------------------- loaders --
     const int lw = warp - 8;
     uint32_t pend0 = 0, pend1 = 0;                       // barriers of the copy groups in flight, oldest first
@@ -134,7 +145,7 @@ paged_tc_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w,
     int used = 0, tiles = 0;                             // ring slots and key tiles so far
     auto copy_rows = [&](uint32_t dst, const T* src, int64_t off) {   // this warp's 32 rows, off: this lane's row
       constexpr int C = D / 8;                           // 16-byte pieces of a row
-#pragma unroll
+#pragma unroll 4
       for (int i = 0; i < C; ++i) {
         const int r = (i * 32 + lane) / C, c = (i * 32 + lane) % C;
         const int64_t o = __shfl_sync(0xffffffffu, off, r);
@@ -142,41 +153,68 @@ paged_tc_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w,
         pt_copy16(dst + (c >> 3) * 16384 + row * 128 + (((c & 7) ^ (row & 7)) << 4), src + (o >= 0 ? o + c * 8 : 0), o >= 0 ? 16 : 0);
       }
     };
-    auto into_ring = [&](const T* src, int64_t off) -> bool {
-      const int slot = used % kRing;
-      if (!wait_for(bar_empty0 + 8 * slot, ((used / kRing) & 1) ^ 1u)) return false;
-      copy_rows(base + Cfg::kOffRing + slot * Cfg::kTile, src, off);
-      push(bar_full0 + 8 * slot);
-      ++used;
-      return true;
-    };
+    const int box = lane / Cfg::kChunks;                 // of a tile that comes by TMA, and its slice of head_dim: this lane's
     bool ok = true;
     for (int tn = 0; ok && iter.next(p, it); ++tn) {
       const int n = max(subtile_tiles(p, it, 0), subtile_tiles(p, it, 1));
       if (n == 0) { --tn; continue; }                    // no key: the softmax warps write zeros
       const int32_t* table = p.tables + (int64_t)it.r * p.width;
-      const int64_t head = (int64_t)it.hk * p.sc.h;
-      auto page_at = [&](int kt) {                       // of this lane's row of the tile; -1: none
-        const int key = kt * kPtKT + lw * 32 + lane;
-        if (kt >= it.k0 + n || key >= it.keys) return -1;
-        const int page = table[p.page.div((uint32_t)key)];
-        if ((unsigned)page < (unsigned)p.n_pages) return page;
+      auto whole = [&](int kt) { return box_rows > 0 && (kt + 1) * kPtKT <= it.keys; };   // comes by TMA
+      // This lane's page of a tile (its box's or its row's) and the first row there.
+      auto key_at = [&](int kt) { return kt * kPtKT + (whole(kt) ? box * box_rows : lw * 32 + lane); };
+      auto page_at = [&](int kt) {
+        if (kt >= it.k0 + n || (whole(kt) && (lw > 0 || box * box_rows >= kPtKT))) return 0;
+        const int key = key_at(kt);
+        return key < it.keys ? table[p.page.div((uint32_t)key)] : -1;
+      };
+      auto there = [&](int page) {
+        if ((unsigned)page < (unsigned)p.n_pages) return true;
         if (p.flag) atomicMax(p.flag, kPagedFlag);
-        return -1;
+        return false;
       };
-      auto row_at = [&](int kt, int page) -> int64_t {
-        const uint32_t key = (uint32_t)(kt * kPtKT + lw * 32 + lane);
-        return page >= 0 ? (int64_t)page * p.sc.b + (int64_t)(key - p.page.div(key) * p.page.d) * p.sc.s + head : -1;
+      // One ring slot: the tile's keys or values, page: as page_at said.
+      auto load = [&](const CUtensorMap* map, const T* pool, int kt, int page, bool keys) -> bool {
+        const int slot = used % kRing;
+        const uint32_t full = bar_full0 + 8 * slot, dst = base + Cfg::kOffRing + slot * Cfg::kTile;
+        if (!wait_for(bar_empty0 + 8 * slot, ((used / kRing) & 1) ^ 1u)) return false;
+        ++used;
+        const int key = key_at(kt);
+        const int in_page = key - (int)(p.page.div((uint32_t)key) * p.page.d);
+        volatile uint32_t* mask = masks + (tiles & 15) * 4;
+        if (keys) ++tiles;
+        if (whole(kt)) {
+          if (lw > 0) {
+            if (lane == 0) mbar_arrive(full);
+            return true;
+          }
+          if (keys) {
+            const uint32_t ok_boxes = __ballot_sync(0xffffffffu, box * box_rows >= kPtKT || there(page));
+            if (lane < 4) {
+              uint32_t m = 0xffffffffu;
+              if (ok_boxes != 0xffffffffu)
+                for (int i = 0; i < 32; ++i)
+                  if (!((ok_boxes >> ((lane * 32 + i) / box_rows * Cfg::kChunks)) & 1)) m &= ~(1u << i);
+              mask[lane] = m;
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_expect_tx(full, Cfg::kTile);
+          __syncwarp();
+          if (box * box_rows < kPtKT)
+            tma_load_4d(dst + (lane % Cfg::kChunks) * 16384 + box * box_rows * 128, map, full, (lane % Cfg::kChunks) * 64, in_page, it.hk, page);
+          return true;
+        }
+        const int64_t off = key < it.keys && there(page) ? (int64_t)page * p.sc.b + (int64_t)in_page * p.sc.s + (int64_t)it.hk * p.sc.h : -1;
+        if (keys) {
+          const uint32_t m = __ballot_sync(0xffffffffu, off >= 0);
+          if (lane == 0) mask[lw] = m;
+        }
+        copy_rows(dst, pool, off);
+        push(full);
+        return true;
       };
-      auto load_k = [&](int64_t off) -> bool {
-        const uint32_t mask = __ballot_sync(0xffffffffu, off >= 0);
-        if (lane == 0) masks[(tiles & 15) * 4 + lw] = mask;
-        ++tiles;
-        return into_ring((const T*)p.kp, off);
-      };
-      int64_t off = row_at(it.k0, page_at(it.k0)), off_next = -1;
-      int page = page_at(it.k0 + 1);
-      if (!(ok = load_k(off))) break;
+      int page = page_at(it.k0), next = page_at(it.k0 + 1);
+      if (!(ok = load(&tmK, (const T*)p.kp, it.k0, page, true))) break;
       // queries, once the last score MMA of the item before has read them
       if (tn > 0 && !(ok = wait_for(bar_qfree, (tn - 1) & 1))) break;
 #pragma unroll 1
@@ -197,13 +235,14 @@ paged_tc_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w,
       }
       push(bar_q);
       for (int i = 0; i < n; ++i) {
+        const int kt = it.k0 + i, page_next = next;
         if (i + 1 < n) {
-          off_next = row_at(it.k0 + i + 1, page);
-          page = page_at(it.k0 + i + 2);
-          if (!(ok = load_k(off_next))) break;
+          next = page_at(kt + 2);
+          if (!(ok = load(&tmK, (const T*)p.kp, kt + 1, page_next, true))) break;
         }
-        if (!(ok = into_ring((const T*)p.vp, off))) break;
-        off = off_next;
+        if (!(ok = load(&tmV, (const T*)p.vp, kt, page, false))) break;
+        page = page_next;
+        if (i == 0) drain();                             // the queries are on their way since before this tile's values
       }
     }
     drain();
@@ -212,27 +251,22 @@ paged_tc_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w,
     if (lane == 0) {
       const uint32_t idesc_s = idesc_f16(is_bf16, 0, 0, 128, 128);
       const uint32_t idesc_o = idesc_f16(is_bf16, 0, 1, 128, D);
-      uint64_t dq[4 * Cfg::kChunks], dk0[4 * Cfg::kChunks], dv0[8];     // of Q_A and of ring slot 0
-#pragma unroll
-      for (int c = 0; c < Cfg::kChunks; ++c)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          dq[c * 4 + k] = smem_desc_sw128(base + c * 16384 + k * 32, 16, 1024);
-          dk0[c * 4 + k] = smem_desc_sw128(base + Cfg::kOffRing + c * 16384 + k * 32, 16, 1024);
-        }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) dv0[k] = smem_desc_sw128(base + Cfg::kOffRing + k * 2048, 16384, 1024);
+      // descriptors of Q_A and of ring slot 0; the others are offsets (in 16-byte units) from these
+      const uint64_t dq = smem_desc_sw128(base, 16, 1024), dk0 = smem_desc_sw128(base + Cfg::kOffRing, 16, 1024),
+                     dv0 = smem_desc_sw128(base + Cfg::kOffRing, 16384, 1024);
       int used = 0, np[2] = {0, 0};                      // ring slots taken; weight tiles awaited per subtile
       auto wait_full = [&](int u) { return mbar_wait(bar_full0 + 8 * (u % kRing), (u / kRing) & 1, abort_flag); };
       auto issue_s = [&](int s, int slot) {
-        uint64_t a[4 * Cfg::kChunks], b[4 * Cfg::kChunks];
 #pragma unroll
-        for (int k = 0; k < 4 * Cfg::kChunks; ++k) {
-          a[k] = dq[k] + (uint64_t)(s * Cfg::kTile >> 4);
-          b[k] = dk0[k] + (uint64_t)(slot * Cfg::kTile >> 4);
+        for (int c = 0; c < Cfg::kChunks; ++c) {
+          uint64_t a[4], b[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            a[k] = dq + (uint32_t)((s * Cfg::kTile + c * 16384 + k * 32) >> 4);
+            b[k] = dk0 + (uint32_t)((slot * Cfg::kTile + c * 16384 + k * 32) >> 4);
+          }
+          umma_f16_x4(tmem_base + 128 * s, a, b, idesc_s, c > 0 ? 1u : 0u);
         }
-        umma_f16_x4(tmem_base + 128 * s, a, b, idesc_s, 0u);
-        if (Cfg::kChunks == 2) umma_f16_x4(tmem_base + 128 * s, a + 4 * (Cfg::kChunks - 1), b + 4 * (Cfg::kChunks - 1), idesc_s, 1u);
         umma_commit(bar_s0 + 8 * s);
       };
       bool ok = true;
@@ -251,9 +285,6 @@ paged_tc_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w,
           const bool more = i + 1 < n;
           if (more) uk = used++;
           const int uv = used++;
-          uint64_t b[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) b[k] = dv0[k] + (uint64_t)((uv % kRing) * Cfg::kTile >> 4);
           if (more && !wait_full(uk)) { ok = false; break; }
           if (!wait_full(uv)) { ok = false; break; }
           for (int s = 0; s < 2; ++s) {
@@ -261,6 +292,9 @@ paged_tc_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w,
             if (!mbar_wait(bar_p0 + 8 * s, np[s] & 1, abort_flag)) { ok = false; break; }
             ++np[s];
             tc_fence_after();
+            uint64_t b[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) b[k] = dv0 + (uint32_t)(((uv % kRing) * Cfg::kTile + k * 2048) >> 4);
             umma_f16_ts_x8(tmem_base + Cfg::kColO + D * s, tmem_base + 128 * s, b, idesc_o, i > 0 ? 1u : 0u);
             if (i + 1 < count[s]) issue_s(s, uk % kRing);
             else umma_commit(bar_o0 + 8 * s);            // the subtile's last product
@@ -276,8 +310,10 @@ paged_tc_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w,
       // the last commit signals shared memory: not after the CTA is gone
       if (used > 0) mbar_wait(bar_empty0 + 8 * ((used - 1) % kRing), ((used - 1) / kRing) & 1, abort_flag);
     }
+  }
   } else {
     // ------------------------------------------------------------- softmax --
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPtRegsMore));
     const int sub = warp >> 2, qtr = warp & 3;
     const int row = sub * 128 + qtr * 32 + lane;         // of the item
     const uint32_t lanes = (uint32_t)(qtr * 32) << 16;
@@ -312,24 +348,21 @@ paged_tc_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w,
             if (left < 32) there[c] &= left <= 0 ? 0u : (1u << left) - 1;
           }
         }
-        uint32_t r[32];
+        uint32_t r[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(tmem_s + 32 * c, r + 32 * c);
+        tmem_ld_wait();
+        if (!full) {
+#pragma unroll
+          for (int e = 0; e < 128; ++e) if (!((there[e >> 5] >> (e & 31)) & 1)) r[e] = 0xff800000u;
+        }
         float x0 = -INFINITY, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (!full && !__any_sync(0xffffffffu, there[c] != 0)) continue;
-          tmem_ld32(tmem_s + 32 * c, r);
-          tmem_ld_wait();
-          if (!full) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) if (!((there[c] >> e) & 1)) r[e] = 0xff800000u;
-          }
-#pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            x0 = max3(x0, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
-            x1 = max3(x1, __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
-            x2 = max3(x2, __uint_as_float(r[e + 4]), __uint_as_float(r[e + 5]));
-            x3 = max3(x3, __uint_as_float(r[e + 6]), __uint_as_float(r[e + 7]));
-          }
+        for (int e = 0; e < 128; e += 8) {
+          x0 = max3(x0, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+          x1 = max3(x1, __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
+          x2 = max3(x2, __uint_as_float(r[e + 4]), __uint_as_float(r[e + 5]));
+          x3 = max3(x3, __uint_as_float(r[e + 6]), __uint_as_float(r[e + 7]));
         }
         const float top = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * p.scale_log2;
         const bool move = top > m && (m == -INFINITY || top - m > 8.f);
@@ -338,12 +371,13 @@ paged_tc_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w,
           if (move) { m = top; l *= c; }
           if (i > 0) {                                   // these scores were issued behind the last product into O
 #pragma unroll 1
-            for (int d = 0; d < D; d += 32) {
-              tmem_ld32(tmem_o + d, r);
+            for (int d = 0; d < D; d += 16) {
+              uint32_t o[16];
+              tmem_ld16(tmem_o + d, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * c);
-              tmem_st32(tmem_o + d, r);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * c);
+              tmem_st16(tmem_o + d, o);
             }
           }
         }
@@ -352,26 +386,15 @@ paged_tc_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w,
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t pk[16];
-          if (full || __any_sync(0xffffffffu, there[c] != 0)) {
-            tmem_ld32(tmem_s + 32 * c, r);
-            tmem_ld_wait();
-            if (!full) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) if (!((there[c] >> e) & 1)) r[e] = 0xff800000u;
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float p0 = ex2_approx(fmaf(__uint_as_float(r[2 * e]), p.scale_log2, -sub_m));
-              const float p1 = ex2_approx(fmaf(__uint_as_float(r[2 * e + 1]), p.scale_log2, -sub_m));
-              l0 += p0;
-              l1 += p1;
-              pk[e] = pack2<T>(p0, p1);
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) pk[e] = 0u;
+          for (int e = 0; e < 16; ++e) {
+            const float p0 = ex2_approx(fmaf(__uint_as_float(r[32 * c + 2 * e]), p.scale_log2, -sub_m));
+            const float p1 = ex2_approx(fmaf(__uint_as_float(r[32 * c + 2 * e + 1]), p.scale_log2, -sub_m));
+            l0 += p0;
+            l1 += p1;
+            pk[e] = pack2<T>(p0, p1);
           }
-          tmem_st16(tmem_s + 16 * c, pk);                // over scores that this thread has read
+          tmem_st16(tmem_s + 16 * c, pk);                // over the scores
         }
         l += l0 + l1;
         tmem_st_wait();
@@ -389,9 +412,23 @@ paged_tc_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w,
       const int slot = partial_slot(it);
       const float inv = l == 0.f ? 0.f : 1.f / l;
       bool nan = false;
-      T* op = (T*)p.o + (real ? (int64_t)(it.x.q0 + token) * p.so.s + (int64_t)h * p.so.h : 0);
-      float* po = w.o + ((int64_t)max(slot, 0) * kPtM + row) * D;
       if (busy) {
+        // Rows leave through the warp's staging buffer, 128 bytes of each at a time, so that eight lanes write them
+        // together (a thread storing its own row piece by piece touched 32 lines per store: 8000 cycles per item).
+        uint8_t* stage = smem_raw + Cfg::kOffStage + warp * 4096;
+        auto flush = [&](auto&& address) {               // address(row of the warp): where its 128 bytes go, null: nowhere
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int rr = j * 4 + (lane >> 3), c = lane & 7;
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((c ^ (rr & 7)) << 4));
+            uint8_t* to = address(rr);
+            if (to) *reinterpret_cast<uint4*>(to + c * 16) = v;
+          }
+          __syncwarp();
+        };
+        const int64_t o_row = real ? (int64_t)(it.x.q0 + token) * p.so.s + (int64_t)h * p.so.h : -1;
+        const int first = sub * 128 + qtr * 32;          // the warp's first row of the item
 #pragma unroll 1
         for (int d = 0; d < D; d += 32) {
           uint32_t r[32];
@@ -402,25 +439,31 @@ paged_tc_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w,
 #pragma unroll
             for (int e = 0; e < 32; ++e) r[e] = 0u;
           }
-          if (!real) continue;
           if (slot >= 0) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<float4*>(po + d + e) = make_float4(__uint_as_float(r[e]), __uint_as_float(r[e + 1]),
-                                                                   __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
+            for (int c = 0; c < 8; ++c)
+              *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
+            float* po = w.o + ((int64_t)slot * kPtM + first) * D + d;
+            flush([&](int rr) { return first + rr < it.rows ? reinterpret_cast<uint8_t*>(po + (int64_t)rr * D) : nullptr; });
             continue;
           }
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
+          for (int c = 0; c < 4; ++c) {
             float v[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) { v[u] = __uint_as_float(r[e + u]) * inv; nan |= isnan(v[u]); }
-            if (o_vec)
-              *reinterpret_cast<uint4*>(op + d + e) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
-            else
-              for (int u = 0; u < 8; ++u) op[d + e + u] = from_f<T>(v[u]);
+            for (int u = 0; u < 8; ++u) { v[u] = __uint_as_float(r[8 * c + u]) * inv; nan |= isnan(v[u]); }
+            *reinterpret_cast<uint4*>(stage + lane * 128 + ((((d & 32) / 8 + c) ^ (lane & 7)) << 4)) =
+                make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+            if (!o_vec && real)                          // rows at any address
+              for (int u = 0; u < 8; ++u) ((T*)p.o)[o_row + d + 8 * c + u] = from_f<T>(v[u]);
           }
+          if (o_vec && (d & 32))
+            flush([&](int rr) {
+              const int64_t at = __shfl_sync(0xffffffffu, o_row, rr);
+              return at >= 0 ? reinterpret_cast<uint8_t*>((T*)p.o + at + d - 32) : nullptr;
+            });
         }
+        nan &= real;
         if (slot >= 0 && real)
           *reinterpret_cast<float2*>(w.ml + ((int64_t)slot * kPtM + row) * 2) = make_float2(m, l);
         uint32_t again = __ballot_sync(0xffffffffu, nan);
@@ -453,8 +496,23 @@ static int launch_paged_tc(const PagedAttnParams& p, cudaStream_t st) {
   if (!part.ok()) return MT_ERR_CUDA;
   const WorkPartials w = partials_in(part.ptr, grid, kPtM, D);
   auto vec = [](const void* x, mt_strides3 s) { return aligned16(x) && s.h % 8 == 0 && s.s % 8 == 0; };
-  MT_CHECK_CUDA(launch_overlapped(kern, dim3((unsigned)grid), dim3(kPtThreads), Cfg::kSmem, st, p, w, 3, tile_slope<kPtM, kPtKT>(p.group),
-                                  std::is_same<T, __nv_bfloat16>::value, vec(p.q, p.sq), vec(p.o, p.so)));
+  const int bf16 = std::is_same<T, __nv_bfloat16>::value;
+  // pages as boxes of a tensor map {head_dim, row, head, page}, whose strides are multiples of one another
+  CUtensorMap tk{}, tv{};
+  const int64_t page = p.page.d;
+  int box_rows = 0;
+  if ((page % 128 == 0 || (page >= 8 && 128 % page == 0)) && p.sc.s > 0 && p.sc.h > 0 && p.sc.b > 0 && p.sc.h % p.sc.s == 0 &&
+      p.sc.b % p.sc.h == 0 && p.sc.b < (1ll << 38) && p.n_pages > 0) {
+    box_rows = page < 128 ? (int)page : 128;
+    const uint64_t dims[4] = {(uint64_t)D, (uint64_t)page, (uint64_t)p.kv_heads, (uint64_t)p.n_pages};
+    const uint64_t strides[3] = {(uint64_t)p.sc.s, (uint64_t)p.sc.h, (uint64_t)p.sc.b};
+    const uint32_t box[4] = {64, (uint32_t)box_rows, 1, 1};
+    int rc;
+    if ((rc = make_tmap_nd(&tk, p.kp, bf16, 4, dims, strides, box))) return rc;
+    if ((rc = make_tmap_nd(&tv, p.vp, bf16, 4, dims, strides, box))) return rc;
+  }
+  MT_CHECK_CUDA(launch_overlapped(kern, dim3((unsigned)grid), dim3(kPtThreads), Cfg::kSmem, st, tk, tv, p, w, 3,
+                                  tile_slope<kPtM, kPtKT>(p.group), bf16, vec(p.q, p.sq), vec(p.o, p.so), box_rows));
   count_launch();
   return launch_join<T, D, kPtM, kPtKT>(p, w, grid, st);
 }

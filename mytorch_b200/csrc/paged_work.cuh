@@ -33,9 +33,10 @@ __device__ __forceinline__ int tile_keys(const PagedAttnParams& p, const PagedRe
 // units of 2^-16.
 template <int KT>
 __device__ __forceinline__ int64_t weight_upto(const PagedRequest& x, uint32_t slope, int T, int nt) {
+  if (nt == 0) return 0;
   const int base = max(x.past, 0) / KT + 1, n = min(T, nt - 1);
   const int64_t w = (int64_t)n * base + (int64_t)(((uint64_t)((int64_t)n * (n + 1)) >> 1) * slope >> 16);
-  return T < nt || nt == 0 ? w : w + base + x.n_new / KT;
+  return T < nt ? w : w + base + x.n_new / KT;
 }
 
 // Exclusive prefix sum of one value per thread and the block's total. `sh`: 33 values.
