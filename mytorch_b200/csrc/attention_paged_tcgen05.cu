@@ -5,7 +5,7 @@
 // 256 query rows (tokens times the query heads of the group, so grouped heads fill tiles and share the loads) of one
 // key/value head, in two subtiles A and B of 128, against key tiles of 128:
 //   warps 8-11  loaders: key and value rows lie wherever their pages are. A tile whose 128 rows are all there
-//               comes by TMA, a box per page (pages of 8 to 128 rows that divide 128, or multiples of 128 rows; zeros for
+//               comes by TMA, in boxes that fill pages (8 rows or more: page sizes that are multiples of 8; zeros for
 //               a page outside the pool); the others, and every tile of odd page sizes, by 16-byte cp.async row by row, with
 //               zeros behind the last key, in the 128-byte swizzle that the MMA reads (it takes a warp 1000 cycles
 //               to queue its 32 rows of one tile, as long as the tile's products run).
@@ -145,12 +145,16 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     int used = 0, tiles = 0;                             // ring slots and key tiles so far
     auto copy_rows = [&](uint32_t dst, const T* src, int64_t off) {   // this warp's 32 rows, off: this lane's row
       constexpr int C = D / 8;                           // 16-byte pieces of a row
-#pragma unroll 4
-      for (int i = 0; i < C; ++i) {
-        const int r = (i * 32 + lane) / C, c = (i * 32 + lane) % C;
-        const int64_t o = __shfl_sync(0xffffffffu, off, r);
-        const int row = lw * 32 + r;
-        pt_copy16(dst + (c >> 3) * 16384 + row * 128 + (((c & 7) ^ (row & 7)) << 4), src + (o >= 0 ? o + c * 8 : 0), o >= 0 ? 16 : 0);
+#pragma unroll
+      for (int i0 = 0; i0 < C; i0 += 8) {                // the exchanges first: one after the other with the copies they take 60 cycles each
+        int64_t o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = __shfl_sync(0xffffffffu, off, ((i0 + i) * 32 + lane) / C);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int c = ((i0 + i) * 32 + lane) % C, row = lw * 32 + ((i0 + i) * 32 + lane) / C;
+          pt_copy16(dst + (c >> 3) * 16384 + row * 128 + (((c & 7) ^ (row & 7)) << 4), src + (o[i] >= 0 ? o[i] + c * 8 : 0), o[i] >= 0 ? 16 : 0);
+        }
       }
     };
     const int box = lane / Cfg::kChunks;                 // of a tile that comes by TMA, and its slice of head_dim: this lane's
@@ -248,50 +252,57 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     drain();
   } else if (warp == 12) {
     // ---------------------------------------------------------- MMA issuer --
-    if (lane == 0) {
-      const uint32_t idesc_s = idesc_f16(is_bf16, 0, 0, 128, 128);
-      const uint32_t idesc_o = idesc_f16(is_bf16, 0, 1, 128, D);
-      // descriptors of Q_A and of ring slot 0; the others are offsets (in 16-byte units) from these
-      const uint64_t dq = smem_desc_sw128(base, 16, 1024), dk0 = smem_desc_sw128(base + Cfg::kOffRing, 16, 1024),
-                     dv0 = smem_desc_sw128(base + Cfg::kOffRing, 16384, 1024);
-      int used = 0, np[2] = {0, 0};                      // ring slots taken; weight tiles awaited per subtile
-      auto wait_full = [&](int u) { return mbar_wait(bar_full0 + 8 * (u % kRing), (u / kRing) & 1, abort_flag); };
-      auto issue_s = [&](int s, int slot) {
+    // The whole warp walks the loop and one lane issues: counts and addresses are the same in all lanes, so that descriptors
+    // are formed on the uniform datapath. (Formed by a thread of its own, the 32 products of a
+    // step took 4500 cycles to issue, twice the time they take to run.)
+    const bool leader = elect_one();
+    const uint32_t idesc_s = idesc_f16(is_bf16, 0, 0, 128, 128);
+    const uint32_t idesc_o = idesc_f16(is_bf16, 0, 1, 128, D);
+    // descriptors of Q_A and of ring slot 0; the others are offsets (in 16-byte units) from these
+    const uint64_t dq = smem_desc_sw128(base, 16, 1024), dk0 = smem_desc_sw128(base + Cfg::kOffRing, 16, 1024),
+                   dv0 = smem_desc_sw128(base + Cfg::kOffRing, 16384, 1024);
+    int used = 0, np[2] = {0, 0};                        // ring slots taken; weight tiles awaited per subtile
+    auto wait_full = [&](int u) { return mbar_wait(bar_full0 + 8 * (u % kRing), (u / kRing) & 1, abort_flag); };
+    auto issue_s = [&](int s, int slot) {                // by the leader
 #pragma unroll
-        for (int c = 0; c < Cfg::kChunks; ++c) {
-          uint64_t a[4], b[4];
+      for (int c = 0; c < Cfg::kChunks; ++c) {
+        uint64_t a[4], b[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            a[k] = dq + (uint32_t)((s * Cfg::kTile + c * 16384 + k * 32) >> 4);
-            b[k] = dk0 + (uint32_t)((slot * Cfg::kTile + c * 16384 + k * 32) >> 4);
-          }
-          umma_f16_x4(tmem_base + 128 * s, a, b, idesc_s, c > 0 ? 1u : 0u);
+        for (int k = 0; k < 4; ++k) {
+          a[k] = dq + (uint32_t)((s * Cfg::kTile + c * 16384 + k * 32) >> 4);
+          b[k] = dk0 + (uint32_t)((slot * Cfg::kTile + c * 16384 + k * 32) >> 4);
         }
-        umma_commit(bar_s0 + 8 * s);
-      };
-      bool ok = true;
-      for (int tn = 0; ok && iter.next(p, it); ++tn) {
-        const int count[2] = {subtile_tiles(p, it, 0), subtile_tiles(p, it, 1)};
-        const int n = max(count[0], count[1]);
-        if (n == 0) { --tn; continue; }
-        int uk = used++;                                 // slot of the next key tile
-        if (!wait_full(uk) || !mbar_wait(bar_q, tn & 1, abort_flag)) break;
-        tc_fence_after();
-        for (int s = 0; s < 2; ++s)
-          if (count[s] > 0) issue_s(s, uk % kRing);
+        umma_f16_x4(tmem_base + 128 * s, a, b, idesc_s, c > 0 ? 1u : 0u);
+      }
+      umma_commit(bar_s0 + 8 * s);
+    };
+    bool ok = true;
+    for (int tn = 0; ok && iter.next(p, it); ++tn) {
+      const int count[2] = {__shfl_sync(0xffffffffu, subtile_tiles(p, it, 0), 0), __shfl_sync(0xffffffffu, subtile_tiles(p, it, 1), 0)};
+      const int n = max(count[0], count[1]);
+      if (n == 0) { --tn; continue; }
+      int uk = used++;                                   // slot of the next key tile
+      if (!__all_sync(0xffffffffu, wait_full(uk) && mbar_wait(bar_q, tn & 1, abort_flag))) break;
+      tc_fence_after();
+      if (leader) {
+        if (count[0] > 0) issue_s(0, uk % kRing);
+        if (count[1] > 0) issue_s(1, uk % kRing);
         umma_commit(bar_empty0 + 8 * (uk % kRing));
         if (n == 1) umma_commit(bar_qfree);
-        for (int i = 0; i < n; ++i) {
-          const bool more = i + 1 < n;
-          if (more) uk = used++;
-          const int uv = used++;
-          if (more && !wait_full(uk)) { ok = false; break; }
-          if (!wait_full(uv)) { ok = false; break; }
-          for (int s = 0; s < 2; ++s) {
-            if (i >= count[s]) continue;
-            if (!mbar_wait(bar_p0 + 8 * s, np[s] & 1, abort_flag)) { ok = false; break; }
-            ++np[s];
-            tc_fence_after();
+      }
+      __syncwarp();
+      for (int i = 0; i < n; ++i) {
+        const bool more = i + 1 < n;
+        if (more) uk = used++;
+        const int uv = used++;
+        if (!__all_sync(0xffffffffu, (!more || wait_full(uk)) && wait_full(uv))) { ok = false; break; }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (i >= count[s]) continue;
+          if (!__all_sync(0xffffffffu, mbar_wait(bar_p0 + 8 * s, np[s] & 1, abort_flag))) { ok = false; break; }
+          ++np[s];
+          tc_fence_after();
+          if (leader) {
             uint64_t b[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) b[k] = dv0 + (uint32_t)(((uv % kRing) * Cfg::kTile + k * 2048) >> 4);
@@ -299,17 +310,21 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             if (i + 1 < count[s]) issue_s(s, uk % kRing);
             else umma_commit(bar_o0 + 8 * s);            // the subtile's last product
           }
-          if (!ok) break;
+          __syncwarp();
+        }
+        if (!ok) break;
+        if (leader) {
           umma_commit(bar_empty0 + 8 * (uv % kRing));
           if (more) {
             umma_commit(bar_empty0 + 8 * (uk % kRing));
             if (i + 2 == n) umma_commit(bar_qfree);      // the item's last score MMA
           }
         }
+        __syncwarp();
       }
-      // the last commit signals shared memory: not after the CTA is gone
-      if (used > 0) mbar_wait(bar_empty0 + 8 * ((used - 1) % kRing), ((used - 1) / kRing) & 1, abort_flag);
     }
+    // the last commit signals shared memory: not after the CTA is gone
+    if (used > 0) mbar_wait(bar_empty0 + 8 * ((used - 1) % kRing), ((used - 1) / kRing) & 1, abort_flag);
   }
   } else {
     // ------------------------------------------------------------- softmax --
@@ -501,9 +516,10 @@ static int launch_paged_tc(const PagedAttnParams& p, cudaStream_t st) {
   CUtensorMap tk{}, tv{};
   const int64_t page = p.page.d;
   int box_rows = 0;
-  if ((page % 128 == 0 || (page >= 8 && 128 % page == 0)) && p.sc.s > 0 && p.sc.h > 0 && p.sc.b > 0 && p.sc.h % p.sc.s == 0 &&
+  const int64_t fits = page % 128 == 0 ? 128 : page & -page;   // largest power of two in page: a box never leaves its page
+  if (fits >= 8 && p.sc.s > 0 && p.sc.h > 0 && p.sc.b > 0 && p.sc.h % p.sc.s == 0 &&
       p.sc.b % p.sc.h == 0 && p.sc.b < (1ll << 38) && p.n_pages > 0) {
-    box_rows = page < 128 ? (int)page : 128;
+    box_rows = fits < 128 ? (int)fits : 128;
     const uint64_t dims[4] = {(uint64_t)D, (uint64_t)page, (uint64_t)p.kv_heads, (uint64_t)p.n_pages};
     const uint64_t strides[3] = {(uint64_t)p.sc.s, (uint64_t)p.sc.h, (uint64_t)p.sc.b};
     const uint32_t box[4] = {64, (uint32_t)box_rows, 1, 1};
