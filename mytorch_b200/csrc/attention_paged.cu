@@ -1,33 +1,6 @@
-// Attention of every request's new rows over the pages of its key/value cache (mt_attn_paged).
+// C entry point of attention over pages: argument checks and the choice of the kernel, by the rows (new tokens times the query
+// heads of the group) that the caller expects per key/value head.
 #include "attention_paged.cuh"
-#include "paged_work.cuh"
-
-namespace mt {
-
-template <typename T, int D>
-__global__ void __launch_bounds__(128)
-paged_plain_kernel(const __grid_constant__ PagedAttnParams p) {
-  const int64_t at = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const int token = (int)(at / p.heads), h = (int)(at % p.heads);
-  if (token >= p.rows || token < p.starts[0] || token >= p.starts[p.requests]) return;
-  int lo = 0, hi = p.requests;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.starts[mid] <= token) lo = mid; else hi = mid;
-  }
-  const PagedRequest x = paged_request(p, lo);
-  if (token - x.q0 < x.n_new) paged_row_plain<T, D>(p, x, lo, token - x.q0, h);
-}
-
-template <typename T, int D>
-static int launch_plain(const PagedAttnParams& p, cudaStream_t st) {
-  const int64_t warps = (int64_t)p.rows * p.heads;
-  paged_plain_kernel<T, D><<<(unsigned)((warps + 3) / 4), 128, 0, st>>>(p);
-  MT_LAUNCH_CHECK();
-  return MT_OK;
-}
-
-}  // namespace mt
 
 using namespace mt;
 
@@ -67,9 +40,7 @@ int mt_attn_paged(const void* q, const void* k_pages, const void* v_pages, void*
   cudaStream_t st = as_stream(stream);
   const int64_t row_hint = (max_new < rows ? max_new : rows) * p.group;
   if (row_hint <= (dtype == MT_F32 ? 8 : 32)) return attn_paged_few(p, row_hint, (int)head_dim, dtype, st);
-  if (dtype != MT_F32) return attn_paged_tc(p, (int)head_dim, dtype, st);
-  MT_DISPATCH_FLOAT(dtype, T, return head_dim == 64 ? (launch_plain<T, 64>(p, st)) : (launch_plain<T, 128>(p, st)));
-  return MT_OK;
+  return dtype == MT_F32 ? attn_paged_f32(p, (int)head_dim, st) : attn_paged_tc(p, (int)head_dim, dtype, st);
 }
 
 }  // extern "C"
