@@ -202,7 +202,7 @@ paged_few_half_kernel(const __grid_constant__ PagedAttnParams p, const WorkParti
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dependency_wait();
   allow_dependents();
-  const WorkShare share = find_share<M, Cfg::KT>(p, least, slope);
+  const WorkShare share = find_share<M, Cfg::KT, 1, 8>(p, least, slope);
   publish_share(share, w);
   FewLoader<T, D, M> load;
   load.ring = smem_addr(few_smem) + warp * Cfg::kRing;
@@ -412,7 +412,7 @@ paged_few_f32_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartia
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dependency_wait();
   allow_dependents();
-  const WorkShare share = find_share<M, Cfg::KT>(p, least, slope);
+  const WorkShare share = find_share<M, Cfg::KT, 1, 8>(p, least, slope);
   publish_share(share, w);
   FewLoader<T, D, M> load;
   load.ring = smem_addr(few_smem) + warp * Cfg::kRing;

@@ -4,13 +4,14 @@
 // Persistent, one CTA per SM, 512 threads; a CTA walks its share of the work (paged_work.cuh). An item is
 // 256 query rows (tokens times the query heads of the group, so grouped heads fill tiles and share the loads) of one
 // key/value head, in two subtiles A and B of 128, against key tiles of 128:
-//   warps 8-11  loaders: key and value rows lie wherever their pages are. A tile whose 128 rows are all there
-//               comes by TMA, in boxes that fill pages (8 rows or more: page sizes that are multiples of 8; zeros for
-//               a page outside the pool); the others, and every tile of odd page sizes, by 16-byte cp.async row by row, with
-//               zeros behind the last key, in the 128-byte swizzle that the MMA reads (it takes a warp 1000 cycles
-//               to queue its 32 rows of one tile, as long as the tile's products run).
-//               One ring in the order of use, K0 K1 V0 K2 V1 ...; page lookups run a tile ahead; which of a tile's rows
-//               are there is a mask next to it.
+//   warps 8-11  loaders: key and value rows lie wherever their pages are. They come by TMA (queued by warp 8) in boxes that fill
+//               pages, 8 rows or more: page sizes that are multiples of 8; zeros for a page outside the pool. Behind the
+//               last key a page's rows may hold anything: warps 9-11 clear such rows of the values before
+//               the MMA sees them (keys are masked as scores). Other page sizes come by 16-byte cp.async, row by row, in the
+//               128-byte swizzle that the MMA reads (it takes a warp 1000 cycles to queue its 32 rows of a tile, as long as
+//               the tile's products run). Queries are a box where the heads of a group divide 128, else rows
+//               as well. One ring in the order of use, K0 K1 V0 K2 V1 ...; page lookups run a tile ahead; which of a tile's
+//               rows are there is a mask next to it.
 //   warp 12     MMA issuer: S_A = Q_A K^T and S_B = Q_B K^T into tensor memory, then per tile O_A += P_A V and the
 //               next S_A while subtile B is in its softmax, O_B += P_B V and the next S_B while A is: the
 //               tensor pipe always has the other subtile's products.
@@ -39,6 +40,7 @@ constexpr int kPtThreads = 512;
 constexpr int kPtRegsMore = 184, kPtRegsLess = 72;
 static_assert(kPtRegsMore + kPtRegsLess <= 2 * 128, "more registers than the block was launched with");
 constexpr int kPtAbort = 105;
+constexpr int kPtFixed = 4, kPtNear = 16;
 
 template <int D> struct PtCfg {
   static constexpr int kChunks = D / 64;                 // 64-column (128-byte) slices of head_dim
@@ -46,8 +48,8 @@ template <int D> struct PtCfg {
   static constexpr int kRing = D == 128 ? 4 : 8;
   static constexpr int kOffRing = 2 * kTile;             // behind Q_A and Q_B
   static constexpr int kOffBar = kOffRing + kRing * kTile;
-  static constexpr int kOffMask = kOffBar + 256;         // [16 tiles][4 words]
-  static constexpr int kOffStage = kOffMask + 768;       // a softmax warp's 32 rows x 128 bytes on their way out, swizzled
+  static constexpr int kOffMask = kOffBar + 512;         // [16 tiles][4 words]
+  static constexpr int kOffStage = kOffMask + 512;       // a softmax warp's 32 rows x 128 bytes on their way out, swizzled
   static constexpr int kSmem = kOffStage + 8 * 4096;
   static constexpr int kColO = 256;
   static_assert(kSmem + 1024 <= 232448, "shared memory of one CTA, static part included");
@@ -67,9 +69,9 @@ __device__ __forceinline__ void pt_copy16(uint32_t dst, const void* src, int byt
 
 template <int D, typename T>
 __global__ void __launch_bounds__(kPtThreads, 1)
-paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                const __grid_constant__ PagedAttnParams p, const WorkPartials w, int least, uint32_t slope, int is_bf16, int q_vec,
-                int o_vec, int box_rows) {
+paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                const __grid_constant__ CUtensorMap tmO, const __grid_constant__ PagedAttnParams p, const WorkPartials w, int least, uint32_t slope, int is_bf16, int q_vec,
+                int q_box, int o_vec, int o_box, int box_rows) {
   using Cfg = PtCfg<D>;
   constexpr int kRing = Cfg::kRing;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -80,13 +82,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   }
   const uint32_t bar0 = base + Cfg::kOffBar;
   const uint32_t bar_full0 = bar0, bar_empty0 = bar0 + 64, bar_q = bar0 + 128, bar_qfree = bar0 + 136, bar_s0 = bar0 + 144,
-                 bar_p0 = bar0 + 160, bar_o0 = bar0 + 176;
+                 bar_p0 = bar0 + 160, bar_o0 = bar0 + 176, bar_tail0 = bar0 + 256;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_raw + Cfg::kOffBar + 192);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_raw + Cfg::kOffBar + 196);
   volatile uint32_t* masks = reinterpret_cast<volatile uint32_t*>(smem_raw + Cfg::kOffMask);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kRing; ++i) { mbar_init(bar_full0 + 8 * i, 4); mbar_init(bar_empty0 + 8 * i, 1); }
+    for (int i = 0; i < kRing; ++i) { mbar_init(bar_full0 + 8 * i, 4); mbar_init(bar_empty0 + 8 * i, 1); mbar_init(bar_tail0 + 8 * i, 1); }
     mbar_init(bar_q, 4);
     mbar_init(bar_qfree, 1);
     for (int s = 0; s < 2; ++s) { mbar_init(bar_s0 + 8 * s, 1); mbar_init(bar_p0 + 8 * s, 4); mbar_init(bar_o0 + 8 * s, 1); }
@@ -100,7 +102,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   }
   grid_dependency_wait();
   allow_dependents();
-  const WorkShare share = find_share<kPtM, kPtKT>(p, least, slope);
+  const WorkShare share = find_share<kPtM, kPtKT, kPtFixed, kPtNear>(p, least, slope);
   publish_share(share, w);
   tc_fence_before();
   __syncthreads();
@@ -158,16 +160,16 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
       }
     };
     const int box = lane / Cfg::kChunks;                 // of a tile that comes by TMA, and its slice of head_dim: this lane's
+    uint32_t cleared = 0;                                // by slot: parity of the tiles with rows to clear
     bool ok = true;
     for (int tn = 0; ok && iter.next(p, it); ++tn) {
       const int n = max(subtile_tiles(p, it, 0), subtile_tiles(p, it, 1));
       if (n == 0) { --tn; continue; }                    // no key: the softmax warps write zeros
       const int32_t* table = p.tables + (int64_t)it.r * p.width;
-      auto whole = [&](int kt) { return box_rows > 0 && (kt + 1) * kPtKT <= it.keys; };   // comes by TMA
       // This lane's page of a tile (its box's or its row's) and the first row there.
-      auto key_at = [&](int kt) { return kt * kPtKT + (whole(kt) ? box * box_rows : lw * 32 + lane); };
+      auto key_at = [&](int kt) { return kt * kPtKT + (box_rows > 0 ? box * box_rows : lw * 32 + lane); };
       auto page_at = [&](int kt) {
-        if (kt >= it.k0 + n || (whole(kt) && (lw > 0 || box * box_rows >= kPtKT))) return 0;
+        if (kt >= it.k0 + n || (box_rows > 0 && (lw > 0 || box * box_rows >= kPtKT))) return -1;
         const int key = key_at(kt);
         return key < it.keys ? table[p.page.div((uint32_t)key)] : -1;
       };
@@ -178,7 +180,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
       };
       // One ring slot: the tile's keys or values, page: as page_at said.
       auto load = [&](const CUtensorMap* map, const T* pool, int kt, int page, bool keys) -> bool {
-        const int slot = used % kRing;
+        const int slot = used % kRing, valid = it.keys - kt * kPtKT;       // rows of the tile before the last key
         const uint32_t full = bar_full0 + 8 * slot, dst = base + Cfg::kOffRing + slot * Cfg::kTile;
         if (!wait_for(bar_empty0 + 8 * slot, ((used / kRing) & 1) ^ 1u)) return false;
         ++used;
@@ -186,26 +188,41 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         const int in_page = key - (int)(p.page.div((uint32_t)key) * p.page.d);
         volatile uint32_t* mask = masks + (tiles & 15) * 4;
         if (keys) ++tiles;
-        if (whole(kt)) {
+        if (box_rows > 0) {
+          const bool clear = !keys && valid < kPtKT;     // values behind the last key
+          const uint32_t landed = clear ? bar_tail0 + 8 * slot : full;
           if (lw > 0) {
-            if (lane == 0) mbar_arrive(full);
+            if (clear) {
+              if (!__all_sync(0xffffffffu, mbar_wait(landed, (cleared >> slot) & 1, abort_flag))) return false;
+              cleared ^= 1u << slot;
+              uint8_t* rows = smem_raw + Cfg::kOffRing + slot * Cfg::kTile;
+              for (int i = (lw - 1) * 32 + lane; i < (kPtKT - valid) * Cfg::kChunks * 8; i += 96) {
+                const int row = valid + i / (Cfg::kChunks * 8), c = i % (Cfg::kChunks * 8);
+                *reinterpret_cast<uint4*>(rows + (c >> 3) * 16384 + row * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+              }
+              announce(full);
+            } else if (lane == 0) mbar_arrive(full);
             return true;
           }
           if (keys) {
-            const uint32_t ok_boxes = __ballot_sync(0xffffffffu, box * box_rows >= kPtKT || there(page));
+            const uint32_t boxes = __ballot_sync(0xffffffffu, box * box_rows >= kPtKT || key >= it.keys || there(page));
             if (lane < 4) {
-              uint32_t m = 0xffffffffu;
-              if (ok_boxes != 0xffffffffu)
+              const int left = valid - lane * 32;
+              uint32_t m = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1;
+              if (boxes != 0xffffffffu)
                 for (int i = 0; i < 32; ++i)
-                  if (!((ok_boxes >> ((lane * 32 + i) / box_rows * Cfg::kChunks)) & 1)) m &= ~(1u << i);
+                  if (!((boxes >> ((lane * 32 + i) / box_rows * Cfg::kChunks)) & 1)) m &= ~(1u << i);
               mask[lane] = m;
             }
           }
           __syncwarp();
-          if (lane == 0) mbar_expect_tx(full, Cfg::kTile);
+          if (lane == 0) {
+            mbar_expect_tx(landed, Cfg::kTile);
+            if (clear) mbar_arrive(full);
+          }
           __syncwarp();
           if (box * box_rows < kPtKT)
-            tma_load_4d(dst + (lane % Cfg::kChunks) * 16384 + box * box_rows * 128, map, full, (lane % Cfg::kChunks) * 64, in_page, it.hk, page);
+            tma_load_4d(dst + (lane % Cfg::kChunks) * 16384 + box * box_rows * 128, map, landed, (lane % Cfg::kChunks) * 64, in_page, it.hk, page);
           return true;
         }
         const int64_t off = key < it.keys && there(page) ? (int64_t)page * p.sc.b + (int64_t)in_page * p.sc.s + (int64_t)it.hk * p.sc.h : -1;
@@ -221,6 +238,17 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
       if (!(ok = load(&tmK, (const T*)p.kp, it.k0, page, true))) break;
       // queries, once the last score MMA of the item before has read them
       if (tn > 0 && !(ok = wait_for(bar_qfree, (tn - 1) & 1))) break;
+      if (q_box) {
+        if (lw == 0 && lane == 0) {
+          const int halves = it.rows > 128 ? 2 : 1;
+          mbar_expect_tx(bar_q, halves * Cfg::kTile);
+          for (int s = 0; s < halves; ++s)
+            for (int c = 0; c < Cfg::kChunks; ++c)
+              tma_load_3d(base + s * Cfg::kTile + c * 16384, &tmQ, bar_q, c * 64, it.hk * p.group,
+                          it.x.q0 + (int)p.by_group.div((uint32_t)(it.t * kPtM + s * 128)));
+        } else if (lane == 0) mbar_arrive(bar_q);
+        __syncwarp();
+      } else {
 #pragma unroll 1
       for (int s = 0; s < 2; ++s) {
         const int row = s * 128 + lw * 32 + lane;
@@ -238,6 +266,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         }
       }
       push(bar_q);
+      }
       for (int i = 0; i < n; ++i) {
         const int kt = it.k0 + i, page_next = next;
         if (i + 1 < n) {
@@ -246,7 +275,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         }
         if (!(ok = load(&tmV, (const T*)p.vp, kt, page, false))) break;
         page = page_next;
-        if (i == 0) drain();                             // the queries are on their way since before this tile's values
+        if (i == 0 && !q_box) drain();                   // the queries are on their way since before this tile's values
       }
     }
     drain();
@@ -426,24 +455,15 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
       }
       const int slot = partial_slot(it);
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      bool nan = false;
+      float odd = 0.f;                                   // NaN once an output is NaN or infinite
       if (busy) {
-        // Rows leave through the warp's staging buffer, 128 bytes of each at a time, so that eight lanes write them
-        // together (a thread storing its own row piece by piece touched 32 lines per store: 8000 cycles per item).
+        // Rows leave through the warp's staging buffer (swizzled), 128 bytes of each at a time and as one copy for all 32:
+        // partial results as they lie there (the joining kernel reads them so), outputs through a tensor map
+        // where all 32 rows are the item's and the heads of the group divide 32, else by eight lanes per row. (A thread storing its own
+        // row piece by piece touched 32 lines per store: 8000 cycles per item; eight lanes per row take 5000.)
         uint8_t* stage = smem_raw + Cfg::kOffStage + warp * 4096;
-        auto flush = [&](auto&& address) {               // address(row of the warp): where its 128 bytes go, null: nowhere
-          __syncwarp();
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int rr = j * 4 + (lane >> 3), c = lane & 7;
-            const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((c ^ (rr & 7)) << 4));
-            uint8_t* to = address(rr);
-            if (to) *reinterpret_cast<uint4*>(to + c * 16) = v;
-          }
-          __syncwarp();
-        };
         const int64_t o_row = real ? (int64_t)(it.x.q0 + token) * p.so.s + (int64_t)h * p.so.h : -1;
-        const int first = sub * 128 + qtr * 32;          // the warp's first row of the item
+        const bool boxed = o_box && it.rows >= sub * 128 + qtr * 32 + 32;
 #pragma unroll 1
         for (int d = 0; d < D; d += 32) {
           uint32_t r[32];
@@ -454,34 +474,58 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
 #pragma unroll
             for (int e = 0; e < 32; ++e) r[e] = 0u;
           }
+          if (slot >= 0 || !(d & 32)) {                  // the buffer's last copy has read it
+            if (lane == 0) bulk_wait_read<0>();
+            __syncwarp();
+          }
           if (slot >= 0) {
 #pragma unroll
             for (int c = 0; c < 8; ++c)
               *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
-            float* po = w.o + ((int64_t)slot * kPtM + first) * D + d;
-            flush([&](int rr) { return first + rr < it.rows ? reinterpret_cast<uint8_t*>(po + (int64_t)rr * D) : nullptr; });
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              bulk_store_1d(w.o + partial_at<D>(slot, sub * 128 + qtr * 32, d), smem_u32(stage), 4096);
+              bulk_commit();
+            }
             continue;
           }
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             float v[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) { v[u] = __uint_as_float(r[8 * c + u]) * inv; nan |= isnan(v[u]); }
+            for (int u = 0; u < 8; ++u) { v[u] = __uint_as_float(r[8 * c + u]) * inv; odd = fmaf(v[u], 0.f, odd); }
             *reinterpret_cast<uint4*>(stage + lane * 128 + ((((d & 32) / 8 + c) ^ (lane & 7)) << 4)) =
                 make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
             if (!o_vec && real)                          // rows at any address
               for (int u = 0; u < 8; ++u) ((T*)p.o)[o_row + d + 8 * c + u] = from_f<T>(v[u]);
           }
-          if (o_vec && (d & 32))
-            flush([&](int rr) {
-              const int64_t at = __shfl_sync(0xffffffffu, o_row, rr);
-              return at >= 0 ? reinterpret_cast<uint8_t*>((T*)p.o + at + d - 32) : nullptr;
-            });
+          if (!o_vec || !(d & 32)) continue;
+          if (boxed) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_3d(&tmO, smem_u32(stage), d - 32, it.hk * p.group, it.x.q0 + token);
+              bulk_commit();
+            }
+            continue;
+          }
+          __syncwarp();
+#pragma unroll 2
+          for (int j = 0; j < 8; ++j) {
+            const int rr = j * 4 + (lane >> 3), c = lane & 7;
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((c ^ (rr & 7)) << 4));
+            const int64_t at = __shfl_sync(0xffffffffu, o_row, rr);
+            if (at >= 0) *reinterpret_cast<uint4*>((T*)p.o + at + d - 32 + c * 8) = v;
+          }
+          __syncwarp();
         }
-        nan &= real;
+        const bool nan = real && isnan(odd);
         if (slot >= 0 && real)
           *reinterpret_cast<float2*>(w.ml + ((int64_t)slot * kPtM + row) * 2) = make_float2(m, l);
         uint32_t again = __ballot_sync(0xffffffffu, nan);
+        if (again && lane == 0) bulk_wait_all<0>();      // before these rows are written once more
+        __syncwarp();
         while (again) {
           const int at = __ffs((int)again) - 1;
           again &= again - 1;
@@ -490,6 +534,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
       }
       tc_fence_before();                                 // O is read: the next item's weights may follow
     }
+    if (lane == 0) bulk_wait_all<0>();                   // the copies must be done with shared memory before the CTA exits
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
@@ -512,23 +558,33 @@ static int launch_paged_tc(const PagedAttnParams& p, cudaStream_t st) {
   const WorkPartials w = partials_in(part.ptr, grid, kPtM, D);
   auto vec = [](const void* x, mt_strides3 s) { return aligned16(x) && s.h % 8 == 0 && s.s % 8 == 0; };
   const int bf16 = std::is_same<T, __nv_bfloat16>::value;
+  CUtensorMap tq{}, tk{}, tv{}, to{};
+  int rc;
   // pages as boxes of a tensor map {head_dim, row, head, page}, whose strides are multiples of one another
-  CUtensorMap tk{}, tv{};
-  const int64_t page = p.page.d;
+  const int64_t page = p.page.d, fits = page % 128 == 0 ? 128 : page & -page;   // largest power of two in page: a box never leaves its page
   int box_rows = 0;
-  const int64_t fits = page % 128 == 0 ? 128 : page & -page;   // largest power of two in page: a box never leaves its page
-  if (fits >= 8 && p.sc.s > 0 && p.sc.h > 0 && p.sc.b > 0 && p.sc.h % p.sc.s == 0 &&
-      p.sc.b % p.sc.h == 0 && p.sc.b < (1ll << 38) && p.n_pages > 0) {
+  if (fits >= 8 && p.sc.s > 0 && p.sc.h > 0 && p.sc.b > 0 && p.sc.h % p.sc.s == 0 && p.sc.b % p.sc.h == 0 && p.sc.b < (1ll << 38) &&
+      p.n_pages > 0) {
     box_rows = fits < 128 ? (int)fits : 128;
     const uint64_t dims[4] = {(uint64_t)D, (uint64_t)page, (uint64_t)p.kv_heads, (uint64_t)p.n_pages};
     const uint64_t strides[3] = {(uint64_t)p.sc.s, (uint64_t)p.sc.h, (uint64_t)p.sc.b};
     const uint32_t box[4] = {64, (uint32_t)box_rows, 1, 1};
-    int rc;
     if ((rc = make_tmap_nd(&tk, p.kp, bf16, 4, dims, strides, box))) return rc;
     if ((rc = make_tmap_nd(&tv, p.vp, bf16, 4, dims, strides, box))) return rc;
   }
-  MT_CHECK_CUDA(launch_overlapped(kern, dim3((unsigned)grid), dim3(kPtThreads), Cfg::kSmem, st, tk, tv, p, w, 3,
-                                  tile_slope<kPtM, kPtKT>(p.group), bf16, vec(p.q, p.sq), vec(p.o, p.so), box_rows));
+  // query and output rows as boxes {head_dim, heads of a group, tokens} of 128 and 32 rows
+  auto rows_map = [&](CUtensorMap* m, int* on, const void* x, mt_strides3 s, int rows) {
+    *on = vec(x, s) && rows % p.group == 0 && s.h > 0 && s.s > 0 && s.s % s.h == 0 && s.s < (1ll << 38);
+    if (!*on) return (int)MT_OK;
+    const uint64_t dims[3] = {(uint64_t)D, (uint64_t)p.heads, (uint64_t)p.rows};
+    const uint64_t strides[2] = {(uint64_t)s.h, (uint64_t)s.s};
+    const uint32_t box[3] = {64, (uint32_t)p.group, (uint32_t)(rows / p.group)};
+    return make_tmap_nd(m, x, bf16, 3, dims, strides, box);
+  };
+  int q_box, o_box;
+  if ((rc = rows_map(&tq, &q_box, p.q, p.sq, 128)) || (rc = rows_map(&to, &o_box, p.o, p.so, 32))) return rc;
+  MT_CHECK_CUDA(launch_overlapped(kern, dim3((unsigned)grid), dim3(kPtThreads), Cfg::kSmem, st, tq, tk, tv, to, p, w, 3,
+                                  tile_slope<kPtM, kPtKT>(p.group), bf16, vec(p.q, p.sq), q_box, vec(p.o, p.so), o_box, box_rows));
   count_launch();
   return launch_join<T, D, kPtM, kPtKT>(p, w, grid, st);
 }

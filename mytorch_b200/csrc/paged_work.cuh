@@ -28,13 +28,13 @@ __device__ __forceinline__ int tile_keys(const PagedAttnParams& p, const PagedRe
 }
 
 // Weight of the first T of nt tiles of one head, in key tiles: increasing, in closed form and free of
-// divisions (a block's first 2 us are this arithmetic, and every block does it). A tile's weight is one for
-// its fixed cost (queries in, output out) and the keys that its rows see; `slope` is what a tile sees more than the one before, M / (group * KT), in
+// divisions (a block's first 2 us are this arithmetic, and every block does it). A tile's weight is FIXED for
+// queries in and output out, and the keys that its rows see; `slope` is what a tile sees more than the one before, M / (group * KT), in
 // units of 2^-16.
-template <int KT>
+template <int KT, int FIXED>
 __device__ __forceinline__ int64_t weight_upto(const PagedRequest& x, uint32_t slope, int T, int nt) {
   if (nt == 0) return 0;
-  const int base = max(x.past, 0) / KT + 1, n = min(T, nt - 1);
+  const int base = max(x.past, 0) / KT + FIXED, n = min(T, nt - 1);
   const int64_t w = (int64_t)n * base + (int64_t)(((uint64_t)((int64_t)n * (n + 1)) >> 1) * slope >> 16);
   return T < nt ? w : w + base + x.n_new / KT;
 }
@@ -62,9 +62,10 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t& t
 struct WorkShare { WorkPos begin; const WorkPos* end; int blocks; };    // blocks that have work
 
 // This block's share (valid until the block ends: `end` is in shared memory); every thread calls it and gets
-// the same answer. `least`: at least so many key tiles per block, fixed costs included. Threads sum up the
+// the same answer. `least`: at least so many key tiles per block, fixed costs included. Cuts nearer to an item's ends
+// than 1/NEAR of a share move there. Threads sum up the
 // weights of their requests; then warp 0 finds where the share begins and warp 1 where it ends.
-template <int M, int KT>
+template <int M, int KT, int FIXED, int NEAR>
 __device__ __forceinline__ WorkShare find_share(const PagedAttnParams& p, int least, uint32_t slope) {
   __shared__ int64_t sums[33];
   __shared__ int64_t before[2];          // of the two cuts: weights before the thread's requests
@@ -76,13 +77,13 @@ __device__ __forceinline__ WorkShare find_share(const PagedAttnParams& p, int le
   for (int r = r0; r < r1; ++r) {
     const PagedRequest x = paged_request(p, r);
     const int nt = row_tiles<M>(p, x);
-    mine += weight_upto<KT>(x, slope, nt, nt) * p.kv_heads;
+    mine += weight_upto<KT, FIXED>(x, slope, nt, nt) * p.kv_heads;
   }
   if (threadIdx.x < 2) owner[threadIdx.x] = -1;
   const int64_t at = block_scan(mine, sums, total);
   // Every block computes the same numbers, and rounding keeps the order of the cuts: that is all they need.
   const int blocks = (int)fmaxf(1.f, fminf((float)gridDim.x, (float)total / (float)least));
-  const int snap = (int)fminf(1e9f, (float)total / (float)(8 * blocks));    // cuts this near to an item's ends move there
+  const int snap = (int)fminf(1e9f, (float)total / (float)(NEAR * blocks));
   auto cut_of = [&](int c) { return (int64_t)((float)total * ((float)c / (float)blocks)); };
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
@@ -100,7 +101,7 @@ __device__ __forceinline__ WorkShare find_share(const PagedAttnParams& p, int le
       for (f.r = owner[e];; ++f.r) {
         x = paged_request(p, f.r);
         nt = row_tiles<M>(p, x);
-        head = weight_upto<KT>(x, slope, nt, nt);
+        head = weight_upto<KT, FIXED>(x, slope, nt, nt);
         if (cut < head * p.kv_heads) break;
         cut -= head * p.kv_heads;
       }
@@ -111,9 +112,9 @@ __device__ __forceinline__ WorkShare find_share(const PagedAttnParams& p, int le
       int lo = 0, hi = nt;                           // the last tile that begins at or before the cut
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (weight_upto<KT>(x, slope, mid, nt) <= cut) lo = mid; else hi = mid;
+        if (weight_upto<KT, FIXED>(x, slope, mid, nt) <= cut) lo = mid; else hi = mid;
       }
-      const int64_t begin = weight_upto<KT>(x, slope, lo, nt), width = weight_upto<KT>(x, slope, lo + 1, nt) - begin;
+      const int64_t begin = weight_upto<KT, FIXED>(x, slope, lo, nt), width = weight_upto<KT, FIXED>(x, slope, lo + 1, nt) - begin;
       const int n = (tile_keys<M>(p, x, lo) + KT - 1) / KT;
       const int kt = min(n - 1, (int)((float)(cut - begin) * (float)n / (float)width));
       f.t = lo;
@@ -173,13 +174,26 @@ struct WorkIter {
 };
 
 // Partial results of a block's first and last item, where a cut runs through them: [2 per block][M rows]
-// of D sums, then the rows' maxima (log2 domain) and weights' sums; `cuts`: where every block begins, the number of
+// of D sums (laid out by partial_row), then the rows' maxima (log2 domain) and weights' sums; `cuts`: where every block begins, the number of
 // blocks with work behind the last.
 struct WorkPartials {
   float* o;
   float* ml;
   WorkPos* cuts;
 };
+
+// Where the tensor-core kernel (256 rows) keeps 32 rows' columns [col, col + 32) of a partial result, in floats from
+// the start: 32 rows of 128 bytes, whose 16-byte pieces lie swizzled by row as its staging buffers have them.
+template <int D>
+__device__ __forceinline__ int64_t partial_at(int slot, int row, int col) {
+  return (((int64_t)slot * 8 + row / 32) * (D / 32) + col / 32) * 1024;
+}
+// E neighbouring columns of a row of a partial result.
+template <int D, int M, int E>
+__device__ __forceinline__ int64_t partial_row(int slot, int row, int col) {
+  if (M < 256) return ((int64_t)slot * M + row) * D + col;
+  return partial_at<D>(slot, row, col) + (row & 31) * 32 + ((((col & 31) >> 2) ^ (row & 7)) << 2) + (col & 3);
+}
 
 __device__ __forceinline__ int partial_slot(const WorkItem& it) {
   return it.k0 > 0 ? 2 * (int)blockIdx.x : it.k1 < it.n ? 2 * (int)blockIdx.x + 1 : -1;
@@ -327,7 +341,7 @@ paged_join_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials 
         const int s = __shfl_sync(0xffffffffu, slot, k);
         const float f = __shfl_sync(0xffffffffu, a, k);
         struct alignas(4 * E) Pack { float t[E]; } v{};
-        if (s >= 0) v = *reinterpret_cast<const Pack*>(w.o + ((int64_t)s * M + row) * D + lane * E);
+        if (s >= 0) v = *reinterpret_cast<const Pack*>(w.o + partial_row<D, M, E>(s, row, lane * E));
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = fmaf(v.t[e], f, o[e]);
       }
