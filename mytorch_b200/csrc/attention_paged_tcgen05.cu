@@ -4,14 +4,14 @@
 // Persistent, one CTA per SM, 512 threads; a CTA walks its share of the work (paged_work.cuh). An item is
 // 256 query rows (tokens times the query heads of the group, so grouped heads fill tiles and share the loads) of one
 // key/value head, in two subtiles A and B of 128, against key tiles of 128:
-//   warps 8-11  loaders: key and value rows lie wherever their pages are. They come by TMA (queued by warp 8) in boxes that fill
-//               pages, 8 rows or more: page sizes that are multiples of 8; zeros for a page outside the pool. Behind the
-//               last key a page's rows may hold anything: warps 9-11 clear such rows of the values before
-//               the MMA sees them (keys are masked as scores). Other page sizes come by 16-byte cp.async, row by row, in the
-//               128-byte swizzle that the MMA reads (it takes a warp 1000 cycles to queue its 32 rows of a tile, as long as
-//               the tile's products run). Queries are a box where the heads of a group divide 128, else rows
-//               as well. One ring in the order of use, K0 K1 V0 K2 V1 ...; page lookups run a tile ahead; which of a tile's
-//               rows are there is a mask next to it.
+//   warps 8-11  loaders: key and value rows lie wherever their pages are. They come by TMA in boxes that fill pages, 8 rows or
+//               more (page sizes that are multiples of 8; zeros for a page outside the pool), each warp a quarter of a tile's
+//               boxes: one warp alone takes 5000 cycles to queue the 32 copies of a step with pages of 16 rows, more than the step runs.
+//               Other page sizes come by 16-byte cp.async, row by row, in the 128-byte swizzle that the MMA reads. Queries
+//               are a box where the heads of a group divide 128, else rows as well. One ring in the order of use,
+//               K0 K1 V0 K2 V1 ...; page lookups run a tile ahead; which of a tile's rows are there is a mask next to it.
+//   warps 13-15 clear the values behind the last key, where a page's rows may hold anything, before the MMA sees
+//               them (such keys are masked as scores).
 //   warp 12     MMA issuer: S_A = Q_A K^T and S_B = Q_B K^T into tensor memory, then per tile O_A += P_A V and the
 //               next S_A while subtile B is in its softmax, O_B += P_B V and the next S_B while A is: the
 //               tensor pipe always has the other subtile's products.
@@ -48,7 +48,7 @@ template <int D> struct PtCfg {
   static constexpr int kRing = D == 128 ? 4 : 8;
   static constexpr int kOffRing = 2 * kTile;             // behind Q_A and Q_B
   static constexpr int kOffBar = kOffRing + kRing * kTile;
-  static constexpr int kOffMask = kOffBar + 512;         // [16 tiles][4 words]
+  static constexpr int kOffMask = kOffBar + 512;         // [16 tiles][4 words]: a bit per row, or per box as the loaders share them
   static constexpr int kOffStage = kOffMask + 512;       // a softmax warp's 32 rows x 128 bytes on their way out, swizzled
   static constexpr int kSmem = kOffStage + 8 * 4096;
   static constexpr int kColO = 256;
@@ -88,7 +88,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   volatile uint32_t* masks = reinterpret_cast<volatile uint32_t*>(smem_raw + Cfg::kOffMask);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kRing; ++i) { mbar_init(bar_full0 + 8 * i, 4); mbar_init(bar_empty0 + 8 * i, 1); mbar_init(bar_tail0 + 8 * i, 1); }
+    for (int i = 0; i < kRing; ++i) { mbar_init(bar_full0 + 8 * i, 4); mbar_init(bar_empty0 + 8 * i, 1); mbar_init(bar_tail0 + 8 * i, 4); }
     mbar_init(bar_q, 4);
     mbar_init(bar_qfree, 1);
     for (int s = 0; s < 2; ++s) { mbar_init(bar_s0 + 8 * s, 1); mbar_init(bar_p0 + 8 * s, 4); mbar_init(bar_o0 + 8 * s, 1); }
@@ -159,8 +159,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         }
       }
     };
-    const int box = lane / Cfg::kChunks;                 // of a tile that comes by TMA, and its slice of head_dim: this lane's
-    uint32_t cleared = 0;                                // by slot: parity of the tiles with rows to clear
+    // Boxes of a tile that comes by TMA: lane i of this warp knows the page of box i * 4 + lw.
+    const int box = lane * 4 + lw, boxes = box_rows > 0 ? (kPtKT / box_rows - lw + 3) / 4 : 0;
     bool ok = true;
     for (int tn = 0; ok && iter.next(p, it); ++tn) {
       const int n = max(subtile_tiles(p, it, 0), subtile_tiles(p, it, 1));
@@ -169,7 +169,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       // This lane's page of a tile (its box's or its row's) and the first row there.
       auto key_at = [&](int kt) { return kt * kPtKT + (box_rows > 0 ? box * box_rows : lw * 32 + lane); };
       auto page_at = [&](int kt) {
-        if (kt >= it.k0 + n || (box_rows > 0 && (lw > 0 || box * box_rows >= kPtKT))) return -1;
+        if (kt >= it.k0 + n || (box_rows > 0 && lane >= boxes)) return -1;
         const int key = key_at(kt);
         return key < it.keys ? table[p.page.div((uint32_t)key)] : -1;
       };
@@ -189,40 +189,26 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         volatile uint32_t* mask = masks + (tiles & 15) * 4;
         if (keys) ++tiles;
         if (box_rows > 0) {
-          const bool clear = !keys && valid < kPtKT;     // values behind the last key
-          const uint32_t landed = clear ? bar_tail0 + 8 * slot : full;
-          if (lw > 0) {
-            if (clear) {
-              if (!__all_sync(0xffffffffu, mbar_wait(landed, (cleared >> slot) & 1, abort_flag))) return false;
-              cleared ^= 1u << slot;
-              uint8_t* rows = smem_raw + Cfg::kOffRing + slot * Cfg::kTile;
-              for (int i = (lw - 1) * 32 + lane; i < (kPtKT - valid) * Cfg::kChunks * 8; i += 96) {
-                const int row = valid + i / (Cfg::kChunks * 8), c = i % (Cfg::kChunks * 8);
-                *reinterpret_cast<uint4*>(rows + (c >> 3) * 16384 + row * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-              }
-              announce(full);
-            } else if (lane == 0) mbar_arrive(full);
-            return true;
-          }
+          // values behind the last key: the tile is handed over by the warps that clear them
+          const uint32_t landed = !keys && valid < kPtKT ? bar_tail0 + 8 * slot : full;
           if (keys) {
-            const uint32_t boxes = __ballot_sync(0xffffffffu, box * box_rows >= kPtKT || key >= it.keys || there(page));
-            if (lane < 4) {
-              const int left = valid - lane * 32;
-              uint32_t m = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1;
-              if (boxes != 0xffffffffu)
-                for (int i = 0; i < 32; ++i)
-                  if (!((boxes >> ((lane * 32 + i) / box_rows * Cfg::kChunks)) & 1)) m &= ~(1u << i);
-              mask[lane] = m;
-            }
+            const uint32_t fine = __ballot_sync(0xffffffffu, lane >= boxes || key >= it.keys || there(page));
+            if (lane == 0) mask[lw] = fine;              // bit i: box i * 4 + lw
           }
           __syncwarp();
           if (lane == 0) {
-            mbar_expect_tx(landed, Cfg::kTile);
-            if (clear) mbar_arrive(full);
+            if (boxes > 0) mbar_expect_tx(landed, boxes * box_rows * D * 2);
+            else mbar_arrive(landed);
+          }
+          for (int i = 0; i < boxes; ++i) {
+            const int id = __shfl_sync(0xffffffffu, page, i), row = __shfl_sync(0xffffffffu, in_page, i);
+            if (lane == 0) {
+#pragma unroll
+              for (int c = 0; c < Cfg::kChunks; ++c)
+                tma_load_4d(dst + c * 16384 + (i * 4 + lw) * box_rows * 128, map, landed, c * 64, row, it.hk, id);
+            }
           }
           __syncwarp();
-          if (box * box_rows < kPtKT)
-            tma_load_4d(dst + (lane % Cfg::kChunks) * 16384 + box * box_rows * 128, map, landed, (lane % Cfg::kChunks) * 64, in_page, it.hk, page);
           return true;
         }
         const int64_t off = key < it.keys && there(page) ? (int64_t)page * p.sc.b + (int64_t)in_page * p.sc.s + (int64_t)it.hk * p.sc.h : -1;
@@ -279,6 +265,30 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       }
     }
     drain();
+  } else if (warp > 12) {
+    // ------------------------------------------------------------ clearing --
+    int used = 0;                                        // ring slots so far
+    uint32_t cleared = 0;                                // by slot: parity of the tiles cleared there
+    while (box_rows > 0 && iter.next(p, it)) {
+      const int n = max(subtile_tiles(p, it, 0), subtile_tiles(p, it, 1));
+      if (n == 0) continue;
+      used += 2 * n;
+      const int slot = (used - 1) % kRing, valid = it.keys - (it.k0 + n - 1) * kPtKT;   // the item's last values
+      if (valid >= kPtKT) continue;
+      if (!__all_sync(0xffffffffu, mbar_wait(bar_tail0 + 8 * slot, (cleared >> slot) & 1, abort_flag))) break;
+      cleared ^= 1u << slot;
+      uint8_t* rows = smem_raw + Cfg::kOffRing + slot * Cfg::kTile;
+      for (int i = (warp - 13) * 32 + lane; i < (kPtKT - valid) * Cfg::kChunks * 8; i += 96) {
+        const int row = valid + i / (Cfg::kChunks * 8), c = i % (Cfg::kChunks * 8);
+        *reinterpret_cast<uint4*>(rows + (c >> 3) * 16384 + row * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {                                   // four arrivals from three warps
+        mbar_arrive(bar_full0 + 8 * slot);
+        if (warp == 15) mbar_arrive(bar_full0 + 8 * slot);
+      }
+    }
   } else if (warp == 12) {
     // ---------------------------------------------------------- MMA issuer --
     // The whole warp walks the loop and one lane issues: counts and addresses are the same in all lanes, so that descriptors
@@ -381,25 +391,36 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           if (lane == 0) mbar_arrive(bar_p0 + 8 * sub);
           continue;
         }
-        uint32_t there[4], all = 0xffffffffu;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) { there[c] = masks[((tiles + i) & 15) * 4 + c]; all &= there[c]; }
-        const bool full = all == 0xffffffffu && key0 + kPtKT <= lim_min;
-        if (!full) {
-#pragma unroll
+        volatile const uint32_t* mask = masks + ((tiles + i) & 15) * 4;
+        const bool all = (mask[0] & mask[1] & mask[2] & mask[3]) == 0xffffffffu;
+        if (!all || key0 + kPtKT > lim_min) {
+          // What a row does not see becomes -inf where it lies, in pieces: rare tiles take longer, the others have no code for it.
+#pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             const int left = lim - key0 - 32 * c;        // columns of this piece that the row sees
-            if (left < 32) there[c] &= left <= 0 ? 0u : (1u << left) - 1;
+            uint32_t bits = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1;
+            if (!all) {
+              if (box_rows > 0) {
+                for (int e = 0; e < 32; ++e) {
+                  const int at = (32 * c + e) / box_rows;
+                  if (!((mask[at & 3] >> (at >> 2)) & 1)) bits &= ~(1u << e);
+                }
+              } else bits &= mask[c];
+            }
+            if (__all_sync(0xffffffffu, bits == 0xffffffffu)) continue;
+            uint32_t x[32];
+            tmem_ld32(tmem_s + 32 * c, x);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) if (!((bits >> e) & 1)) x[e] = 0xff800000u;
+            tmem_st32(tmem_s + 32 * c, x);
           }
+          tmem_st_wait();
         }
         uint32_t r[128];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(tmem_s + 32 * c, r + 32 * c);
         tmem_ld_wait();
-        if (!full) {
-#pragma unroll
-          for (int e = 0; e < 128; ++e) if (!((there[e >> 5] >> (e & 31)) & 1)) r[e] = 0xff800000u;
-        }
         float x0 = -INFINITY, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 128; e += 8) {
