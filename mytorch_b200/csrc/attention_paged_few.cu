@@ -94,6 +94,7 @@ struct FewLoader {
 
   __device__ __forceinline__ int first_key(int warp) const { return kt * Cfg::KT + warp * Cfg::kRows; }
   __device__ __forceinline__ void advance(const PagedAttnParams& p, int warp, int lane) {
+#pragma unroll 1
     while (valid && kt >= it.k1) {
       valid = iter.next(p, it);
       if (valid) { kt = it.k0; window = -1; }
@@ -154,6 +155,7 @@ __device__ __forceinline__ void few_finish(const PagedAttnParams& p, const WorkP
                                            Row row_stats, Factor factor) {
   constexpr int E = D / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slot = partial_slot(it);
+#pragma unroll 1
   for (int g = warp; g < it.rows; g += kFewWarps) {
     float top, sum, o[E];
     row_stats(g, top, sum);
@@ -208,7 +210,7 @@ paged_few_half_kernel(const __grid_constant__ PagedAttnParams p, const WorkParti
   load.ring = smem_addr(few_smem) + warp * Cfg::kRing;
   load.masks = masks + warp * Cfg::kStages;
   load.start(p, share, warp, lane);
-#pragma unroll
+#pragma unroll 1
   for (int s = 0; s < Cfg::kStages; ++s) load.issue(p, s, warp, lane);
   WorkIter<M, Cfg::KT> iter;
   iter.start(share);
@@ -242,6 +244,7 @@ paged_few_half_kernel(const __grid_constant__ PagedAttnParams p, const WorkParti
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) acc[n][d][0] = acc[n][d][1] = acc[n][d][2] = acc[n][d][3] = 0.f;
     }
+#pragma unroll 1
     for (int kt = it.k0; kt < it.k1; ++kt) {
       copy_wait<Cfg::kStages - 1>();
       __syncwarp();
@@ -418,7 +421,7 @@ paged_few_f32_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartia
   load.ring = smem_addr(few_smem) + warp * Cfg::kRing;
   load.masks = masks + warp * Cfg::kStages;
   load.start(p, share, warp, lane);
-#pragma unroll
+#pragma unroll 1
   for (int s = 0; s < Cfg::kStages; ++s) load.issue(p, s, warp, lane);
   WorkIter<M, Cfg::KT> iter;
   iter.start(share);
@@ -445,6 +448,7 @@ paged_few_f32_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartia
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[g][e] = 0.f;
     }
+#pragma unroll 1
     for (int kt = it.k0; kt < it.k1; ++kt) {
       copy_wait<Cfg::kStages - 1>();
       __syncwarp();

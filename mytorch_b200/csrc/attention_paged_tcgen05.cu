@@ -200,6 +200,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             if (boxes > 0) mbar_expect_tx(landed, boxes * box_rows * D * 2);
             else mbar_arrive(landed);
           }
+#pragma unroll 1
           for (int i = 0; i < boxes; ++i) {
             const int id = __shfl_sync(0xffffffffu, page, i), row = __shfl_sync(0xffffffffu, in_page, i);
             if (lane == 0) {
@@ -220,49 +221,53 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         push(full);
         return true;
       };
-      int page = page_at(it.k0), next = page_at(it.k0 + 1);
-      if (!(ok = load(&tmK, (const T*)p.kp, it.k0, page, true))) break;
-      // queries, once the last score MMA of the item before has read them
-      if (tn > 0 && !(ok = wait_for(bar_qfree, (tn - 1) & 1))) break;
-      if (q_box) {
-        if (lw == 0 && lane == 0) {
-          const int halves = it.rows > 128 ? 2 : 1;
-          mbar_expect_tx(bar_q, halves * Cfg::kTile);
-          for (int s = 0; s < halves; ++s)
-            for (int c = 0; c < Cfg::kChunks; ++c)
-              tma_load_3d(base + s * Cfg::kTile + c * 16384, &tmQ, bar_q, c * 64, it.hk * p.group,
-                          it.x.q0 + (int)p.by_group.div((uint32_t)(it.t * kPtM + s * 128)));
-        } else if (lane == 0) mbar_arrive(bar_q);
-        __syncwarp();
-      } else {
+      // Pages of the tile whose values are next, of the one behind it and of the one behind that.
+      int page = page_at(it.k0), next = page_at(it.k0 + 1), later = -1;
+      // in the order of use: K0, then K1 V0 K2 V1 ... and the last values (one place in the code that queues a tile)
 #pragma unroll 1
-      for (int s = 0; s < 2; ++s) {
-        const int row = s * 128 + lw * 32 + lane;
-        int token, h;
-        row_of<kPtM>(p, it, row, token, h);
-        const int64_t q = row < it.rows ? (int64_t)(it.x.q0 + token) * p.sq.s + (int64_t)h * p.sq.h : -1;
-        const uint32_t dst = base + s * Cfg::kTile;
-        if (q_vec) copy_rows(dst, (const T*)p.q, q);
-        else {                                           // rows at any address: element by element
-          for (int c = 0; c < D; ++c) {
-            const int r = lw * 32 + lane;
-            T* to = reinterpret_cast<T*>(smem_raw + s * Cfg::kTile + (c >> 6) * 16384 + r * 128 + ((((c >> 3) & 7) ^ (r & 7)) << 4)) + (c & 7);
-            *to = q >= 0 ? ((const T*)p.q)[q + c] : from_f<T>(0.f);
+      for (int u = 0; u < 2 * n; ++u) {
+        const bool last = u == 2 * n - 1, keys = u == 0 || ((u & 1) && !last);
+        const int kt = it.k0 + (keys ? (u + 1) / 2 : last ? n - 1 : u / 2 - 1);
+        if (!(ok = load(keys ? &tmK : &tmV, (const T*)(keys ? p.kp : p.vp), kt, u > 0 && keys ? next : page, keys))) break;
+        if (!keys) { page = next; next = later; }
+        else if (u > 0) later = page_at(kt + 1);
+        if (!q_box && (u == 2 || (last && u == 1))) drain();             // the queries are on their way since before this tile's values
+        if (u > 0) continue;
+        // queries, once the last score MMA of the item before has read them
+        if (tn > 0 && !(ok = wait_for(bar_qfree, (tn - 1) & 1))) break;
+        if (q_box) {
+          if (lw == 0 && lane == 0) {
+            const int halves = it.rows > 128 ? 2 : 1;
+            mbar_expect_tx(bar_q, halves * Cfg::kTile);
+#pragma unroll 1
+            for (int s = 0; s < halves; ++s)
+              for (int c = 0; c < Cfg::kChunks; ++c)
+                tma_load_3d(base + s * Cfg::kTile + c * 16384, &tmQ, bar_q, c * 64, it.hk * p.group,
+                            it.x.q0 + (int)p.by_group.div((uint32_t)(it.t * kPtM + s * 128)));
+          } else if (lane == 0) mbar_arrive(bar_q);
+          __syncwarp();
+        } else {
+#pragma unroll 1
+        for (int s = 0; s < 2; ++s) {
+          const int row = s * 128 + lw * 32 + lane;
+          int token, h;
+          row_of<kPtM>(p, it, row, token, h);
+          const int64_t q = row < it.rows ? (int64_t)(it.x.q0 + token) * p.sq.s + (int64_t)h * p.sq.h : -1;
+          const uint32_t dst = base + s * Cfg::kTile;
+          if (q_vec) copy_rows(dst, (const T*)p.q, q);
+          else {                                           // rows at any address: element by element
+#pragma unroll 1
+            for (int c = 0; c < D; ++c) {
+              const int r = lw * 32 + lane;
+              T* to = reinterpret_cast<T*>(smem_raw + s * Cfg::kTile + (c >> 6) * 16384 + r * 128 + ((((c >> 3) & 7) ^ (r & 7)) << 4)) + (c & 7);
+              *to = q >= 0 ? ((const T*)p.q)[q + c] : from_f<T>(0.f);
+            }
           }
         }
-      }
-      push(bar_q);
-      }
-      for (int i = 0; i < n; ++i) {
-        const int kt = it.k0 + i, page_next = next;
-        if (i + 1 < n) {
-          next = page_at(kt + 2);
-          if (!(ok = load(&tmK, (const T*)p.kp, kt + 1, page_next, true))) break;
+        push(bar_q);
         }
-        if (!(ok = load(&tmV, (const T*)p.vp, kt, page, false))) break;
-        page = page_next;
-        if (i == 0 && !q_box) drain();                   // the queries are on their way since before this tile's values
       }
+      if (!ok) break;
     }
     drain();
   } else if (warp > 12) {
@@ -278,6 +283,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       if (!__all_sync(0xffffffffu, mbar_wait(bar_tail0 + 8 * slot, (cleared >> slot) & 1, abort_flag))) break;
       cleared ^= 1u << slot;
       uint8_t* rows = smem_raw + Cfg::kOffRing + slot * Cfg::kTile;
+#pragma unroll 1
       for (int i = (warp - 13) * 32 + lane; i < (kPtKT - valid) * Cfg::kChunks * 8; i += 96) {
         const int row = valid + i / (Cfg::kChunks * 8), c = i % (Cfg::kChunks * 8);
         *reinterpret_cast<uint4*>(rows + (c >> 3) * 16384 + row * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -330,6 +336,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         if (n == 1) umma_commit(bar_qfree);
       }
       __syncwarp();
+#pragma unroll 1
       for (int i = 0; i < n; ++i) {
         const bool more = i + 1 < n;
         if (more) uk = used++;
@@ -382,6 +389,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       const int lim = real ? visible_keys(it.x, token) : INT32_MAX;
       const int lim_min = __reduce_min_sync(0xffffffffu, lim);
       float m = -INFINITY, l = 0.f;
+#pragma unroll 1
       for (int i = 0; i < count; ++i) {
         const int key0 = (it.k0 + i) * kPtKT;
         if (!__all_sync(0xffffffffu, mbar_wait(bar_s0 + 8 * sub, ns & 1, abort_flag))) { ok = false; break; }
@@ -401,6 +409,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             uint32_t bits = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1;
             if (!all) {
               if (box_rows > 0) {
+#pragma unroll 1
                 for (int e = 0; e < 32; ++e) {
                   const int at = (32 * c + e) / box_rows;
                   if (!((mask[at & 3] >> (at >> 2)) & 1)) bits &= ~(1u << e);
@@ -519,6 +528,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             *reinterpret_cast<uint4*>(stage + lane * 128 + ((((d & 32) / 8 + c) ^ (lane & 7)) << 4)) =
                 make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
             if (!o_vec && real)                          // rows at any address
+#pragma unroll
               for (int u = 0; u < 8; ++u) ((T*)p.o)[o_row + d + 8 * c + u] = from_f<T>(v[u]);
           }
           if (!o_vec || !(d & 32)) continue;

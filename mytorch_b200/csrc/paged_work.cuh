@@ -52,6 +52,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t& t
   __syncthreads();
   int64_t before = 0;
   total = 0;
+#pragma unroll 1
   for (int w = 0; w < warps; ++w) {
     if (w < warp) before += sh[w];
     total += sh[w];
@@ -74,6 +75,7 @@ __device__ __forceinline__ WorkShare find_share(const PagedAttnParams& p, int le
   const int per = (p.requests + (int)blockDim.x - 1) / (int)blockDim.x;
   const int r0 = min(p.requests, (int)threadIdx.x * per), r1 = min(p.requests, r0 + per);
   int64_t mine = 0, total;
+#pragma unroll 1
   for (int r = r0; r < r1; ++r) {
     const PagedRequest x = paged_request(p, r);
     const int nt = row_tiles<M>(p, x);
@@ -98,6 +100,7 @@ __device__ __forceinline__ WorkShare find_share(const PagedAttnParams& p, int le
       int64_t cut = cut_of((int)blockIdx.x + e) - before[e], head = 0;
       PagedRequest x{};
       int nt = 0;
+#pragma unroll 1
       for (f.r = owner[e];; ++f.r) {
         x = paged_request(p, f.r);
         nt = row_tiles<M>(p, x);
@@ -107,9 +110,12 @@ __device__ __forceinline__ WorkShare find_share(const PagedAttnParams& p, int le
       }
       f.hk = (int)__fdividef((float)cut, (float)head);
       cut -= f.hk * head;
+#pragma unroll 1
       for (; cut < 0; cut += head) --f.hk;
+#pragma unroll 1
       for (; cut >= head; cut -= head) ++f.hk;
       int lo = 0, hi = nt;                           // the last tile that begins at or before the cut
+#pragma unroll 1
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (weight_upto<KT, FIXED>(x, slope, mid, nt) <= cut) lo = mid; else hi = mid;
@@ -148,6 +154,7 @@ struct WorkIter {
   __device__ __forceinline__ void start(const WorkShare& s) { cur = s.begin; last = s.end; loaded = -1; nt = 0; }
   __device__ __forceinline__ bool next(const PagedAttnParams& p, WorkItem& it) {
     const WorkPos end = *last;
+#pragma unroll 1
     for (;;) {
       if (cur.r >= p.requests) return false;
       if (cur.r > end.r || (cur.r == end.r && (cur.hk > end.hk || (cur.hk == end.hk && (cur.t > end.t || (cur.t == end.t && cur.kt >= end.kt))))))
@@ -271,6 +278,7 @@ __device__ __noinline__ void paged_row_plain(const PagedAttnParams& p, PagedRequ
 #pragma unroll
   for (int e = 0; e < E; ++e) { q[e] = to_f(qp[e]) * p.scale_log2; o[e] = 0.f; }
   const int n = visible_keys(x, i);
+#pragma unroll 1
   for (int j = 0; j < n; ++j) {
     const int64_t at = paged_row(p, table, j);
     if (at < 0) continue;
@@ -310,6 +318,7 @@ paged_join_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials 
   it.x = paged_request(p, cut.r);
   it.rows = (int)min((int64_t)M, (int64_t)it.x.n_new * p.group - (int64_t)cut.t * M);
   int last = c;                                      // the item's pieces: slot 2c-1, then slots 2j of blocks c..last
+#pragma unroll 1
   for (;;) {
     const int j = last + 1 + lane;
     const bool inside = j < blocks && same_item(w.cuts[j], cut) && w.cuts[j].kt > 0;
@@ -318,10 +327,12 @@ paged_join_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials 
     last += 32;
   }
   const int pieces = last - c + 2;
+#pragma unroll 1
   for (int row = (int)blockIdx.y * 4 + warp; row < it.rows; row += 4 * gridDim.y) {
     float m = -INFINITY, l = 0.f, o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll 1
     for (int i0 = 0; i0 < pieces; i0 += 32) {
       const int i = i0 + lane, j = c + i - 1;
       int slot = i < pieces ? (i == 0 ? 2 * c - 1 : 2 * j) : -1;
