@@ -39,7 +39,20 @@ int mt_attn_paged(const void* q, const void* k_pages, const void* v_pages, void*
   p.flag = device_flag_ptr();
   cudaStream_t st = as_stream(stream);
   const int64_t row_hint = (max_new < rows ? max_new : rows) * p.group;
-  if (row_hint <= (dtype == MT_F32 ? 8 : 32)) return attn_paged_few(p, row_hint, (int)head_dim, dtype, st);
+  const int few = dtype == MT_F32 ? 8 : 32;
+  p.most_rows = INT32_MAX;
+  if (row_hint <= few) return attn_paged_few(p, row_hint, (int)head_dim, dtype, st);
+  // Where most requests bring much less than the largest does (a token each, say, beside pieces of prompts), those whose rows
+  // fit in one small tile go to the kernel for few rows first: in tiles of 256 rows they cost the tensor pipe as much as full
+  // ones (18 requests with a token and 6 with 200..700, 10 heads, 100..2000 keys: 103 us in one kernel, SPLIT_US in two; prompts of
+  // similar lengths would pay 6 us for two launches that find nothing to do).
+  const int64_t small = few == 8 ? (p.group <= 1 ? 1 : p.group <= 2 ? 2 : p.group <= 4 ? 4 : 8) : (p.group + 7) / 8 * 8;
+  if (requests > 1 && max_new < rows && p.group <= few && 2 * rows <= requests * max_new) {
+    PagedAttnParams f = p;
+    f.most_rows = (int)small;
+    if (int rc = attn_paged_few(f, small, (int)head_dim, dtype, st)) return rc;
+    p.least_rows = (int)small + 1;
+  }
   return dtype == MT_F32 ? attn_paged_f32(p, (int)head_dim, st) : attn_paged_tc(p, (int)head_dim, dtype, st);
 }
 

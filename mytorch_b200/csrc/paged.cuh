@@ -24,6 +24,7 @@ struct PagedAttnParams {
   mt_strides3 sq, sc, so;                // q, o: {-, head, row}; pools: {page, head, row}
   const int32_t *tables, *starts, *kv_len;
   int requests, width, rows, heads, kv_heads, group, n_pages;
+  int least_rows, most_rows;             // query rows per key/value head of the requests that a launch works on
   FastDiv page, by_group;
   float scale_log2;
   int q_pairs, o_quads;                  // rows of q on 4-byte, rows of o on 8-byte (16-byte in fp32) boundaries
@@ -41,6 +42,7 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedAttnParams& p, 
   PagedRequest x;
   x.q0 = min(max(a, 0), p.rows);
   x.n_new = min(max(b, x.q0), p.rows) - x.q0;
+  if ((int64_t)x.n_new * p.group < p.least_rows || (int64_t)x.n_new * p.group > p.most_rows) x.n_new = 0;   // another launch's
   x.past = (int)max((int64_t)INT32_MIN / 2, (int64_t)kv - ((int64_t)b - a) + (x.q0 - (int64_t)a));
   x.keys = (int)min((int64_t)max(kv, 0), (int64_t)p.width * p.page.d);
   if (kv > x.keys && p.flag) atomicMax(p.flag, kPagedFlag);
