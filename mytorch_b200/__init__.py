@@ -14,6 +14,7 @@ from .tensor import Tensor, no_grad, zeros, ones, zeros_like, randn, arange
 from . import nn, optim, utils, ops
 from .ops import transpose, permute, chunk, concatenate, stack
 from .accelerate import Accelerator, GradScaler
+from .paged import PagedKVCache
 
 __all__ += ["Tensor", "no_grad", "zeros", "ones", "zeros_like", "randn", "arange", "nn", "optim", "ops",
-            "transpose", "permute", "chunk", "concatenate", "stack", "Accelerator", "GradScaler"]
+            "transpose", "permute", "chunk", "concatenate", "stack", "Accelerator", "GradScaler", "PagedKVCache"]

@@ -12,7 +12,7 @@ from dataclasses import dataclass
 
 import numpy as np
 
-from . import _lib, infer, nn
+from . import _lib, fused_ops, infer, nn, paged
 from .array import DeviceArray, stream
 from .nn import functional as F
 from .tensor import Tensor
@@ -130,6 +130,11 @@ class Attention(nn.Module):
         B, T, _ = qkv.shape
         H, D, E = self.num_heads, self.head_dim, self.embed_dim
         arr = qkv.data
+        if isinstance(cache, paged.PagedKVCache):                  # packed tokens of several requests
+            part = lambda i: DeviceArray(arr.ptr + i * D * arr.itemsize, (T, H, D), arr.dtype, base=arr)
+            st = _lib.Strides3(0, 3 * D, 3 * E)
+            cache.update(part(1), part(2), layer_idx, (st, st))
+            return Tensor(cache.attend(part(0), layer_idx, st).reshape(B, T, E))
         sin = _lib.Strides3(T * 3 * E, 3 * D, 3 * E)               # q/k/v of head h start at h*3D (+0, +D, +2D)
         past = cache.get_seq_len(layer_idx)
         kc, vc, kv_len = cache.update(arr.ptr + D * arr.itemsize, arr.ptr + 2 * D * arr.itemsize, sin, B, H, T, D,
@@ -264,8 +269,26 @@ class GPT2(nn.Module):
         cache._appended = [a + T for a in cache._appended]
         return out
 
+    def _paged(self, input_ids, cache):
+        """Logits [requests, 1, V] behind each request's last new token; input_ids [1, tokens] as announced by
+        cache.begin(). Position rows are gathered by position."""
+        cfg, e = self.config, self.embeddings
+        if Tensor.build_graph_enabled() and any(p.requires_grad for p in self.parameters()):
+            raise NotImplementedError("a paged cache holds no graph: run the forward under no_grad()")
+        cache.check(input_ids.shape, cfg.num_blocks, cfg.num_heads, cfg.embed_dim // cfg.num_heads, cfg.max_seq_len)
+        x = F.embedding(input_ids, e.char_embeddings.weight).data
+        at = fused_ops.fused_embedding_forward(e.position_embeddings.weight.data, cache.position)
+        _lib.add(x.ptr, at.ptr, x.ptr, x.size, x.code, stream())
+        x = Tensor(x)
+        for layer_idx, block in enumerate(self.blocks):
+            x = block(x, cache=cache, layer_idx=layer_idx)
+        last = Tensor(fused_ops.fused_embedding_forward(x.data.reshape(-1, cfg.embed_dim), cache.last_rows))
+        return self.lm_head(self.final_layer_norm(last)).data.reshape(cache.last_rows.size, 1, cfg.vocab_size)
+
     def forward(self, x, cache=None):
-        """Logits; with a `Cache`, (logits, cache) as in gpt2.py:352-374."""
+        """Logits; with a `Cache` (or a paged.PagedKVCache), (logits, cache) as in gpt2.py:352-374."""
+        if isinstance(cache, paged.PagedKVCache):
+            return Tensor(self._paged(x, cache)), cache
         from .utils.checkpoint import checkpoint
         plan = infer.plan_of(self, _plan)
         ids = infer.token_ids(x) if plan is not None else None
@@ -298,9 +321,18 @@ class GPT2(nn.Module):
     def generate(self, input_ids, max_new_tokens, temperature=1.0, top_k=None, use_cache=True, seed=None):
         """Autoregressive sampling as in gpt2_trainer/inference_gpt2.py:137-174: the prompt fills
         the cache, then one token per step; temperature-scaled softmax (optionally restricted to
-        the top_k logits), one draw per sequence on the host; temperature 0 takes the arg-max."""
+        the top_k logits), one draw per sequence on the host; temperature 0 takes the arg-max. Prompts of
+        different lengths (a list of sequences) go through a paged cache and come back as a list."""
         from .tensor import no_grad
         rng = np.random.default_rng(seed)
+        if paged.is_ragged(input_ids):
+            if not use_cache:
+                raise ValueError("prompts of different lengths need the cache")
+            cfg = self.config
+            with no_grad():
+                return paged.generate(lambda ids, cache: self._paged(Tensor(ids), cache), input_ids, max_new_tokens,
+                                      paged.sampler(temperature, top_k, rng),
+                                      paged.cache_for(cfg.num_blocks, cfg.num_heads, cfg.embed_dim // cfg.num_heads))
         ids = np.asarray(input_ids.numpy() if isinstance(input_ids, Tensor) else input_ids, dtype=np.int32)
         cache = Cache(self.config) if use_cache else None
         feed = ids

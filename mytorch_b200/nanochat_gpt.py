@@ -20,7 +20,7 @@ from dataclasses import dataclass
 
 import numpy as np
 
-from . import _lib, infer, nn
+from . import _lib, fused_ops, infer, nn, paged
 from .array import DeviceArray, stream
 from .nn import functional as F
 from .tensor import Tensor
@@ -119,7 +119,11 @@ class Attention(nn.Module):
         v = self.v_proj(x).reshape(B, T, Hk, D)
         cos, sin = cos_sin
         q, k = F.rope_qk_norm(q, k, cos, sin)                    # rotary first, then QK-norm over head_dim: one kernel
-        if cache is not None:
+        if isinstance(cache, paged.PagedKVCache):
+            # the packed new tokens of several requests: their keys and values join the pages, each sees its own request
+            cache.update(k.data.reshape(T, Hk, D), v.data.reshape(T, Hk, D), layer_idx)
+            out = Tensor(cache.attend(q.data.reshape(T, H, D), layer_idx).reshape(B, T, E))
+        elif cache is not None:
             # inference: new keys/values join the cache; the prompt (empty cache) attends causally
             # among its own tokens, later tokens see everything cached (nanochat_gpt.py:126-160)
             past = cache.pos
@@ -253,7 +257,29 @@ class GPT(nn.Module):
         cache._pos += T
         return out
 
+    def _paged(self, input_ids, cache):
+        """Logits [requests, 1, V] behind each request's last new token; input_ids [1, tokens] as announced by
+        cache.begin(). Rotary rows are gathered by position."""
+        cfg = self.config
+        if Tensor.build_graph_enabled() and any(p.requires_grad for p in self.parameters()):
+            raise NotImplementedError("a paged cache holds no graph: run the forward under no_grad()")
+        cache.check(input_ids.shape, cfg.num_blocks, cfg.num_kv_heads, cfg.embed_dim // cfg.num_q_heads, cfg.max_seq_len)
+        cos, sin = (fused_ops.fused_embedding_forward(t, cache.position) for t in (self.cos, self.sin))
+        x = self.embeddings(input_ids)
+        for layer_idx, block in enumerate(self.blocks):
+            x = block(x, (cos, sin), cache=cache, layer_idx=layer_idx)
+        last = Tensor(fused_ops.fused_embedding_forward(x.data.reshape(-1, cfg.embed_dim), cache.last_rows))
+        logits = self.lm_head(norm(last))
+        if cfg.softcap and not self.training:
+            arr = logits.data
+            _lib.softcap(arr.ptr, arr.ptr, arr.size, float(cfg.softcap), arr.code, stream())
+        return logits.data.reshape(cache.last_rows.size, 1, cfg.vocab_size)
+
     def forward(self, input_ids, target_ids=None, cache=None):
+        if isinstance(cache, paged.PagedKVCache):
+            if target_ids is not None:
+                raise ValueError("a paged cache is for inference: no targets")
+            return Tensor(self._paged(input_ids, cache)), cache
         B, T = input_ids.shape
         plan = infer.plan_of(self, _plan) if target_ids is None else None
         ids = infer.token_ids(input_ids) if plan is not None else None
@@ -297,11 +323,21 @@ class GPT(nn.Module):
         return self.forward(Tensor(feed), None, cache=cache)[0].data if out is None else out
 
     def generate(self, input_ids, max_new_tokens, temperature=1.0, top_k=None, seed=None):
-        """Cached autoregressive sampling for one batch of equally long prompts: the prompt fills a
-        KVCache, then one token per step (temperature 0 = arg-max)."""
+        """Cached autoregressive sampling: the prompt fills a KVCache, then one token per step (temperature 0 =
+        arg-max). Prompts of different lengths (a list of sequences) go through a paged cache and come back as a list."""
         from .tensor import no_grad
         cfg = self.config
         rng = np.random.default_rng(seed)
+        if paged.is_ragged(input_ids):
+            was_training = self.training
+            self.eval()
+            with no_grad():
+                out = paged.generate(lambda ids, cache: self._paged(Tensor(ids), cache), input_ids, max_new_tokens,
+                                     paged.sampler(temperature, top_k, rng),
+                                     paged.cache_for(cfg.num_blocks, cfg.num_kv_heads, cfg.embed_dim // cfg.num_q_heads))
+            if was_training:
+                self.train()
+            return out
         ids = np.asarray(input_ids.numpy() if isinstance(input_ids, Tensor) else input_ids, dtype=np.int32)
         cache = KVCache(ids.shape[0], cfg.num_kv_heads, cfg.max_seq_len, cfg.embed_dim // cfg.num_q_heads, cfg.num_blocks)
         was_training = self.training
