@@ -417,7 +417,8 @@ int mt_paged_append(const void* k_new, const void* v_new, void* k_pages, void* v
  * no request has are not written. A row that sees no key, or only scores of -inf, is 0; what a row does not see does not
  * reach it, not even as NaN. Keys on a page outside the pool are left out (status word). max_new: the most
  * new rows a request is expected to have, which only picks the kernel (right for any lengths).
- * head_dim 64 or 128; page strides and pools 16-byte aligned; scale positive. */
+ * head_dim 64 or 128; page strides and pools 16-byte aligned; scale positive; o and q do not overlap.
+ * (As everywhere here, the first call on a device goes before a capture.) */
 int mt_attn_paged(const void* q, const void* k_pages, const void* v_pages, void* o, mt_strides3 sq, mt_strides3 spages,
                   mt_strides3 so, const int32_t* tables, const int32_t* starts, const int32_t* kv_len,
                   int64_t requests, int64_t width, int64_t rows, int64_t max_new, int64_t heads, int64_t kv_heads,

@@ -74,7 +74,7 @@ class DeviceArray:
     __slots__ = ("ptr", "shape", "dtype", "_base", "_owns", "__weakref__")
 
     def __init__(self, ptr, shape, dtype, base=None, owns=False):
-        self.ptr = int(ptr)
+        self.ptr = ptr if type(ptr) is int else int(ptr)
         self.shape = tuple(map(int, shape))
         self.dtype = dtype if dtype in _DT else norm_dtype(dtype)
         self._base = base

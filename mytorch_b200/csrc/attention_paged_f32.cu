@@ -40,7 +40,7 @@ paged_f32_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w
   const int cg = lane & 7, row0 = warp * 16 + (lane >> 3) * 4;        // this thread's first row of the tile
   grid_dependency_wait();
   allow_dependents();
-  const WorkShare share = find_share<kPfM, KT, 1, 8>(p, least, slope);
+  const WorkShare share = find_share<kPfM, KT, 1, 8>(p, least, slope, false);
   publish_share(share, w);
   WorkIter<kPfM, KT> iter;
   iter.start(share);

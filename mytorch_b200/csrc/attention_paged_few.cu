@@ -194,7 +194,7 @@ __device__ __forceinline__ float part_weight(float m, float l, float top) {
 
 template <typename T, int D, int M>
 __global__ void __launch_bounds__(kFewWarps * 32, FewCfg<T, D, M>::kBlocks)
-paged_few_half_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w, int least, uint32_t slope) {
+paged_few_half_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w, int least, uint32_t slope, int whole) {
   using Cfg = FewCfg<T, D, M>;
   constexpr int NT = M / 8, KM = Cfg::kRows / 16, C = Cfg::kChunks;
   extern __shared__ __align__(128) uint8_t few_smem[];
@@ -204,7 +204,7 @@ paged_few_half_kernel(const __grid_constant__ PagedAttnParams p, const WorkParti
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dependency_wait();
   allow_dependents();
-  const WorkShare share = find_share<M, Cfg::KT, 1, 8>(p, least, slope);
+  const WorkShare share = find_share<M, Cfg::KT, 1, 8>(p, least, slope, whole);
   publish_share(share, w);
   FewLoader<T, D, M> load;
   load.ring = smem_addr(few_smem) + warp * Cfg::kRing;
@@ -403,7 +403,7 @@ paged_few_half_kernel(const __grid_constant__ PagedAttnParams p, const WorkParti
 
 template <int D, int M>
 __global__ void __launch_bounds__(kFewWarps * 32, FewCfg<float, D, M>::kBlocks)
-paged_few_f32_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w, int least, uint32_t slope) {
+paged_few_f32_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartials w, int least, uint32_t slope, int whole) {
   using T = float;
   using Cfg = FewCfg<T, D, M>;
   constexpr int E = D / 32, C = Cfg::kChunks;
@@ -415,7 +415,7 @@ paged_few_f32_kernel(const __grid_constant__ PagedAttnParams p, const WorkPartia
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dependency_wait();
   allow_dependents();
-  const WorkShare share = find_share<M, Cfg::KT, 1, 8>(p, least, slope);
+  const WorkShare share = find_share<M, Cfg::KT, 1, 8>(p, least, slope, whole);
   publish_share(share, w);
   FewLoader<T, D, M> load;
   load.ring = smem_addr(few_smem) + warp * Cfg::kRing;
@@ -538,12 +538,15 @@ static int launch_few(const PagedAttnParams& p, cudaStream_t st) {
   static SmemLimit limit;
   if (int rc = limit.raise((const void*)kern, Cfg::kSmem)) return rc;
   const int grid = Cfg::kBlocks * sm_count();
-  TempBuf part(partial_bytes(grid, M, D), st);
+  // Tables that end within a few tiles: no item is cut then, and there is nothing to join (a second launch costs 3 us, as
+  // much as six tiles one after the other).
+  const int whole = (int64_t)p.width * p.page.d <= 6 * Cfg::KT;
+  TempBuf part(whole ? 0 : partial_bytes(grid, M, D), st);
   if (!part.ok()) return MT_ERR_CUDA;
-  const WorkPartials w = partials_in(part.ptr, grid, M, D);
-  MT_CHECK_CUDA(launch_overlapped(kern, dim3((unsigned)grid), dim3(kFewWarps * 32), Cfg::kSmem, st, p, w, 3, tile_slope<M, Cfg::KT>(p.group)));
+  const WorkPartials w = whole ? WorkPartials{} : partials_in(part.ptr, grid, M, D);
+  MT_CHECK_CUDA(launch_overlapped(kern, dim3((unsigned)grid), dim3(kFewWarps * 32), Cfg::kSmem, st, p, w, 3, tile_slope<M, Cfg::KT>(p.group), whole));
   count_launch();
-  return launch_join<T, D, M, Cfg::KT>(p, w, grid, st);
+  return whole ? MT_OK : launch_join<T, D, M, Cfg::KT>(p, w, grid, st);
 }
 
 template <typename T, int D>

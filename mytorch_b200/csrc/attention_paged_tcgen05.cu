@@ -102,7 +102,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   }
   grid_dependency_wait();
   allow_dependents();
-  const WorkShare share = find_share<kPtM, kPtKT, kPtFixed, kPtNear>(p, least, slope);
+  const WorkShare share = find_share<kPtM, kPtKT, kPtFixed, kPtNear>(p, least, slope, false);
   publish_share(share, w);
   tc_fence_before();
   __syncthreads();

@@ -63,45 +63,77 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t& t
 struct WorkShare { WorkPos begin; const WorkPos* end; int blocks; };    // blocks that have work
 
 // This block's share (valid until the block ends: `end` is in shared memory); every thread calls it and gets
-// the same answer. `least`: at least so many key tiles per block, fixed costs included. Cuts nearer to an item's ends
-// than 1/NEAR of a share move there. Threads sum up the
-// weights of their requests; then warp 0 finds where the share begins and warp 1 where it ends.
+// the same answer (`blocks`: thread 0). `least`: at least so many key tiles per block, fixed costs included. Cuts nearer
+// to an item's ends than 1/NEAR of a share move there; with `whole` all do, and no item is cut. Warp 0 finds where the share
+// begins and warp 1 where it ends, each with prefix sums of its own over up to 256 requests (two round trips to memory and 3000
+// cycles less than sums over the block first, which longer lists take).
 template <int M, int KT, int FIXED, int NEAR>
-__device__ __forceinline__ WorkShare find_share(const PagedAttnParams& p, int least, uint32_t slope) {
+__device__ __forceinline__ WorkShare find_share(const PagedAttnParams& p, int least, uint32_t slope, bool whole) {
   __shared__ int64_t sums[33];
   __shared__ int64_t before[2];          // of the two cuts: weights before the thread's requests
   __shared__ int owner[2];
   __shared__ WorkPos found[2];
-  const int per = (p.requests + (int)blockDim.x - 1) / (int)blockDim.x;
-  const int r0 = min(p.requests, (int)threadIdx.x * per), r1 = min(p.requests, r0 + per);
-  int64_t mine = 0, total;
-#pragma unroll 1
-  for (int r = r0; r < r1; ++r) {
-    const PagedRequest x = paged_request(p, r);
-    const int nt = row_tiles<M>(p, x);
-    mine += weight_upto<KT, FIXED>(x, slope, nt, nt) * p.kv_heads;
-  }
-  if (threadIdx.x < 2) owner[threadIdx.x] = -1;
-  const int64_t at = block_scan(mine, sums, total);
+  const int lane = threadIdx.x & 31, e = threadIdx.x >> 5;
+  auto weights = [&](int r0, int r1) {
+    int64_t w = 0;
+#pragma unroll 2
+    for (int r = r0; r < r1; ++r) {
+      const PagedRequest x = paged_request(p, r);
+      const int nt = row_tiles<M>(p, x);
+      w += weight_upto<KT, FIXED>(x, slope, nt, nt) * p.kv_heads;
+    }
+    return w;
+  };
   // Every block computes the same numbers, and rounding keeps the order of the cuts: that is all they need.
-  const int blocks = (int)fmaxf(1.f, fminf((float)gridDim.x, (float)total / (float)least));
-  const int snap = (int)fminf(1e9f, (float)total / (float)(NEAR * blocks));
-  auto cut_of = [&](int c) { return (int64_t)((float)total * ((float)c / (float)blocks)); };
+  auto blocks_of = [&](int64_t total) { return (int)fmaxf(1.f, fminf((float)gridDim.x, (float)total / (float)least)); };
+  auto cut_of = [&](int64_t total, int blocks, int c) { return (int64_t)((float)total * ((float)c / (float)blocks)); };
+  const bool few = p.requests <= 256;
+  int64_t total = 0, cut = 0;
+  int blocks = 0, first = -1;            // first: where the search for the cut starts, in the thread that makes it
+  if (few) {
+    if (e < 2) {
+      const int per = (p.requests + 31) / 32, r0 = min(p.requests, lane * per);
+      const int64_t mine = weights(r0, min(p.requests, r0 + per));
+      int64_t at = mine;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int64_t cut = cut_of((int)blockIdx.x + e);
-    if ((int)blockIdx.x + e < blocks && cut >= at && cut < at + mine) { before[e] = at; owner[e] = r0; }
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t t = __shfl_up_sync(0xffffffffu, at, o);
+        if (lane >= o) at += t;
+      }
+      total = __shfl_sync(0xffffffffu, at, 31);
+      at -= mine;
+      blocks = blocks_of(total);
+      const int c = (int)blockIdx.x + e;
+      cut = cut_of(total, blocks, c) - at;
+      if (c < blocks && cut >= 0 && cut < mine) first = r0;
+    }
+  } else {
+    const int per = (p.requests + (int)blockDim.x - 1) / (int)blockDim.x;
+    const int r0 = min(p.requests, (int)threadIdx.x * per);
+    const int64_t mine = weights(r0, min(p.requests, r0 + per));
+    if (threadIdx.x < 2) owner[threadIdx.x] = -1;
+    const int64_t at = block_scan(mine, sums, total);
+    blocks = blocks_of(total);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int c = (int)blockIdx.x + k;
+      const int64_t x = cut_of(total, blocks, c);
+      if (c < blocks && x >= at && x < at + mine) { before[k] = at; owner[k] = r0; }
+    }
+    __syncthreads();
+    if (e < 2 && lane == 0 && owner[e] >= 0) {
+      first = owner[e];
+      cut = cut_of(total, blocks, (int)blockIdx.x + e) - before[e];
+    }
   }
-  __syncthreads();
-  const int e = threadIdx.x >> 5;
-  if (e < 2 && (threadIdx.x & 31) == 0) {
-    WorkPos f{p.requests, 0, 0, 0};                  // the list's end
-    if (owner[e] >= 0) {
-      int64_t cut = cut_of((int)blockIdx.x + e) - before[e], head = 0;
+  if (e < 2) {
+    if (first >= 0) {
+      int64_t head = 0;
       PagedRequest x{};
+      WorkPos f;
       int nt = 0;
 #pragma unroll 1
-      for (f.r = owner[e];; ++f.r) {
+      for (f.r = first;; ++f.r) {
         x = paged_request(p, f.r);
         nt = row_tiles<M>(p, x);
         head = weight_upto<KT, FIXED>(x, slope, nt, nt);
@@ -123,11 +155,13 @@ __device__ __forceinline__ WorkShare find_share(const PagedAttnParams& p, int le
       const int64_t begin = weight_upto<KT, FIXED>(x, slope, lo, nt), width = weight_upto<KT, FIXED>(x, slope, lo + 1, nt) - begin;
       const int n = (tile_keys<M>(p, x, lo) + KT - 1) / KT;
       const int kt = min(n - 1, (int)((float)(cut - begin) * (float)n / (float)width));
+      const int snap = whole ? n / 2 : (int)fminf(1e9f, (float)total / (float)(NEAR * blocks));
       f.t = lo;
       f.kt = kt <= snap ? 0 : kt;
-      if (f.kt && n - kt <= snap) { ++f.t; f.kt = 0; }
+      if (f.kt && (whole || n - kt <= snap)) { ++f.t; f.kt = 0; }
+      found[e] = f;
     }
-    found[e] = f;
+    if (__ballot_sync(0xffffffffu, first >= 0) == 0 && lane == 0) found[e] = WorkPos{p.requests, 0, 0, 0};   // the list's end
   }
   __syncthreads();
   return WorkShare{found[0], &found[1], blocks};     // without a share both are the list's end
@@ -230,9 +264,9 @@ struct SmemLimit {
   }
 };
 
-// The block whose share begins at blockIdx.x tells the joining kernel so.
+// The block whose share begins at blockIdx.x tells the joining kernel so, if there is one.
 __device__ __forceinline__ void publish_share(const WorkShare& s, const WorkPartials& w) {
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 0 && w.cuts) {
     w.cuts[blockIdx.x] = s.begin;
     if (blockIdx.x == 0) w.cuts[gridDim.x] = WorkPos{s.blocks, 0, 0, 0};
   }

@@ -14,6 +14,7 @@ deliberate and visible to callers:
   * nothing here synchronises with the host.
 """
 import ctypes as C
+import functools
 import math
 
 from . import _lib
@@ -393,9 +394,19 @@ def _pools(k_pages, v_pages):
     return k, v
 
 
-def _page_strides(a):
-    _, H, S, D = a.shape
+@functools.lru_cache(maxsize=None)
+def _page_strides(H, S, D):
     return _lib.Strides3(H * S * D, S * D, D)
+
+
+@functools.lru_cache(maxsize=None)
+def _row_strides(H, D):
+    return _lib.Strides3(0, D, H * D)
+
+
+def _same_float(a, b, c):
+    if not (a.dtype == b.dtype == c.dtype and a.dtype in ("float16", "bfloat16", "float32")):
+        _check_float(a, b, c)
 
 
 def fused_paged_tables(held, fresh, tables, free_pages, n_free, page_size, rows=None, out=None):
@@ -433,13 +444,14 @@ def fused_paged_append(k, v, k_pages, v_pages, slot, strides=None):
     slots are skipped. `strides` (two Strides3, batch unused) reads views such as a fused projection."""
     k, v = _A(k), _A(v)
     k_pages, v_pages = _pools(k_pages, v_pages)
-    _check_float(k, v, k_pages, v_pages)
+    _same_float(k, k_pages, v_pages)
+    _same_float(k, v, v_pages)
     P, H, S, D = k_pages.shape
     if len(k.shape) != 3 or k.shape != v.shape or k.shape[1:] != (H, D):
         raise ValueError(f"new keys and values are [rows, {H}, {D}] both, got {k.shape} and {v.shape}")
     slot = _ints("slot", slot, k.shape[0])
-    sk, sv = strides or (_lib.Strides3(0, D, H * D),) * 2
-    _lib.paged_append(k.ptr, v.ptr, k_pages.ptr, v_pages.ptr, sk, sv, _page_strides(k_pages), slot.ptr, k.shape[0], H, D, S, P,
+    sk, sv = strides or (_row_strides(H, D),) * 2
+    _lib.paged_append(k.ptr, v.ptr, k_pages.ptr, v_pages.ptr, sk, sv, _page_strides(H, S, D), slot.ptr, k.shape[0], H, D, S, P,
                       k.code, stream())
 
 
@@ -451,7 +463,7 @@ def fused_paged_attention(q, k_pages, v_pages, tables, starts, kv_len, max_new=N
     `strides` (Strides3, batch unused) reads q as a view. Not differentiable: a cache holds no graph."""
     q = _A(q)
     k_pages, v_pages = _pools(k_pages, v_pages)
-    _check_float(q, k_pages, v_pages)
+    _same_float(q, k_pages, v_pages)
     P, Hk, S, D = k_pages.shape
     if len(q.shape) != 3 or q.shape[2] != D or q.shape[1] % Hk:
         raise ValueError(f"q is [rows, heads, {D}] with a multiple of {Hk} heads, got {q.shape}")
@@ -465,8 +477,8 @@ def fused_paged_attention(q, k_pages, v_pages, tables, starts, kv_len, max_new=N
         out = _A(out)
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError(f"out is {q.dtype} {q.shape}, got {out.dtype} {out.shape}")
-    row = _lib.Strides3(0, D, H * D)
-    _lib.attn_paged(q.ptr, k_pages.ptr, v_pages.ptr, out.ptr, strides or row, _page_strides(k_pages), row, tables.ptr, starts.ptr,
+    row = _row_strides(H, D)
+    _lib.attn_paged(q.ptr, k_pages.ptr, v_pages.ptr, out.ptr, strides or row, _page_strides(Hk, S, D), row, tables.ptr, starts.ptr,
                     kv_len.ptr, R, tables.shape[1], N, N if max_new is None else max_new, H, Hk, D, S, P,
                     float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(D), q.code, stream())
     return out

@@ -43,11 +43,11 @@ def test_append_refusals(lib):
 
 def test_attention_refusals(lib):
     row, pages = lib.Strides3(0, 64, 256), lib.Strides3(2048, 1024, 64)
-    ok = [A, A, A, A, row, pages, row, A, A, A, 2, 8, 3, 1, 4, 2, 64, 16, 8, 0.125, lib.BF16]
+    ok = [A, A, A, A + 4096, row, pages, row, A, A, A, 2, 8, 3, 1, 4, 2, 64, 16, 8, 0.125, lib.BF16]
     for change, text in [({0: None}, "bad arguments"), ({9: None}, "bad arguments"), ({10: -1}, "bad arguments"), ({14: 3}, "multiple"),
                          ({16: 80}, "head_dim"), ({17: 0}, "positions"), ({11: 1 << 28}, "positions"), ({11: 1 << 62, 17: 4}, "positions"),
                          ({5: lib.Strides3(2048, 1024, 60)}, "16-byte"), ({5: lib.Strides3(2050, 1024, 64)}, "16-byte"), ({1: A + 2}, "16-byte"),
-                         ({19: 0.0}, "scale"), ({19: -1.0}, "scale"), ({19: float("inf")}, "scale"), ({19: float("nan")}, "scale"),
+                         ({3: A}, "of its own"), ({19: 0.0}, "scale"), ({19: -1.0}, "scale"), ({19: float("inf")}, "scale"), ({19: float("nan")}, "scale"),
                          ({20: 5}, "dtype"), ({12: 1 << 30, 14: 4}, "rows"), ({13: -1}, "rows")]:
         refused(lib.attn_paged, [change.get(i, v) for i, v in enumerate(ok)], text, lib)
 

@@ -409,3 +409,48 @@ def test_no_requests_and_no_rows(mt):
     mt.fused_ops.fused_paged_attention(z(0, 1, 64), *pools, i32(mt, np.zeros((1, 1))), i32(mt, [0, 0]), i32(mt, [0]))
     mt.fused_ops.fused_paged_append(z(0, 1, 64), z(0, 1, 64), *pools, i32(mt, np.zeros(0)))
     no_device_flag(mt)
+
+
+# Rows that lie apart from each other, at odd addresses too, and pools with the heads inside a page's rows.
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("max_new", [1, 150])
+@pytest.mark.parametrize("heads,kv_heads,D", [(4, 2, 64), (5, 1, 128), (2, 2, 128)])
+@pytest.mark.parametrize("lead,gap", [(0, 64), (8, 8), (1, 3)])
+@pytest.mark.parametrize("rows_first", [False, True])
+def test_strides(mt, dtype, max_new, heads, kv_heads, D, lead, gap, rows_first):
+    from mytorch_b200 import _lib
+    from mytorch_b200.array import stream
+    step = Step(MIXED, heads, kv_heads, D, 16, dtype, seed=lead)
+    wide = np.full((step.rows, heads * D + gap), 7.0, np.float32)
+    wide[:, :heads * D] = step.q.reshape(step.rows, -1)
+    flat = np.concatenate([np.full(lead, 7.0, np.float32), wide.reshape(-1)])
+    Q, O = dev(mt, flat, dtype), dev(mt, np.full(flat.shape, 7.0), dtype)
+    at, st = lead * Q.itemsize, _lib.Strides3(0, D, heads * D + gap)
+    pools = [p.swapaxes(1, 2) if rows_first else p for p in (step.k, step.v)]
+    K, V = (dev(mt, np.ascontiguousarray(p), dtype) for p in pools)
+    sp = _lib.Strides3(kv_heads * 16 * D, D, kv_heads * D) if rows_first else _lib.Strides3(kv_heads * 16 * D, 16 * D, D)
+    ints = [i32(mt, a) for a in (step.tables, step.starts, [kv for kv, _ in step.requests])]       # kept until the call is queued
+    _lib.attn_paged(Q.ptr + at, K.ptr, V.ptr, O.ptr + at, st, sp, st, *[a.ptr for a in ints], len(step.requests), step.width, step.rows, max_new, heads, kv_heads, D, 16,
+                    step.pages, D ** -0.5, Q.code, stream())
+    flat = O.numpy().astype(np.float64)
+    got = flat[lead:].reshape(step.rows, -1)
+    assert (flat[:lead] == 7).all() and (got[:, heads * D:] == 7).all() and (got[step.starts[-1]:] == 7).all()
+    want, tol = step.want()
+    assert (np.abs(got[:step.starts[-1], :heads * D].reshape(want.shape) - want) <= tol).all()
+    no_device_flag(mt)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("max_new", [1, 50])
+def test_rows_before_the_first_request(mt, dtype, max_new):
+    """starts need not begin at row 0, and a request may end where the rows do."""
+    step = Step([(70, 50), (33, 1), (9, 9)], 4, 2, 64, 16, dtype, pad=0)
+    want, tol = step.want()
+    n = step.rows
+    q = np.concatenate([np.full((5, 4, 64), np.nan, np.float32), step.q])
+    O = dev(mt, np.full(q.shape, 7.0), dtype)
+    mt.fused_ops.fused_paged_attention(dev(mt, q, dtype), dev(mt, step.k, dtype), dev(mt, step.v, dtype), i32(mt, step.tables),
+                                       i32(mt, step.starts + 5), i32(mt, [kv for kv, _ in step.requests]), max_new=max_new, out=O)
+    got = O.numpy()
+    assert (got[:5] == 7).all() and (np.abs(got[5:] - want) <= tol).all() and len(got) == n + 5
+    no_device_flag(mt)
