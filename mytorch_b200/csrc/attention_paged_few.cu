@@ -23,7 +23,7 @@ namespace mt {
 
 constexpr int kFewWarps = 4;
 
-// M rows per item: 8, 16, 24 or 32 in half precision, 1, 2, 4 or 8 in fp32.
+// M rows per item: 8 or 16 in half precision, 1, 2, 4 or 8 in fp32.
 template <typename T, int D, int M> struct FewCfg {
   static constexpr bool kHalf = sizeof(T) == 2;
   static constexpr int kRows = kHalf ? (D == 64 ? 32 : 16) : 8;  // keys of a warp in a tile
@@ -553,9 +553,10 @@ template <typename T, int D>
 static int launch_few_rows(const PagedAttnParams& p, int64_t rows, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {
     if (rows <= 8) return launch_few<T, D, 8>(p, st);
-    if (rows <= 16) return launch_few<T, D, 16>(p, st);
-    if (rows <= 24) return launch_few<T, D, 24>(p, st);
-    return launch_few<T, D, 32>(p, st);
+    // More rows than 16 read keys and values again (from L2) for each 16: tiles of 24 and 32 rows need 255 registers and take
+    // longer where latency counts (20 rows, 16 x 500..2000 keys x 128: 26.6 us against 22.7; 28 rows, 8 x 200..900: 29.3 against
+    // 19.2) and gain 7 % where bandwidth does (20 rows, 64 requests: 43.0 against 46.1).
+    return launch_few<T, D, 16>(p, st);
   } else {
     if (rows <= 1) return launch_few<T, D, 1>(p, st);
     if (rows <= 2) return launch_few<T, D, 2>(p, st);
