@@ -44,11 +44,12 @@ int mt_attn_paged(const void* q, const void* k_pages, const void* v_pages, void*
   p.most_rows = INT32_MAX;
   if (row_hint <= few) return attn_paged_few(p, row_hint, (int)head_dim, dtype, st);
   // Where most requests bring much less than the largest does (a token each, say, beside pieces of prompts), those whose rows
-  // fit in one small tile go to the kernel for few rows first: in tiles of 256 rows they cost the tensor pipe as much as full
-  // ones (18 requests with a token and 6 with 200..700, 10 heads, 100..2000 keys: 103 us in one kernel, SPLIT_US in two; prompts of
-  // similar lengths would pay 6 us for two launches that find nothing to do).
+  // fit in one small tile can go to the kernel for few rows first: a tile of many rows takes its time whatever is in it. At
+  // head_dim 128 that time is about what its keys and values take to arrive, and one launch is better (24 requests, 10
+  // heads: 95 us against 101; 64 requests, 10/2 heads: 72 against 81); at 64 and in fp32 it is not (64 requests, 12 heads of 64, fp16: 101 us
+  // against 74 in two; 24 in fp32: 210 against 133).
   const int64_t small = few == 8 ? (p.group <= 1 ? 1 : p.group <= 2 ? 2 : p.group <= 4 ? 4 : 8) : (p.group + 7) / 8 * 8;
-  if (requests > 1 && max_new < rows && p.group <= few && 2 * rows <= requests * max_new) {
+  if ((head_dim == 64 || dtype == MT_F32) && requests > 1 && max_new < rows && p.group <= few && 2 * rows <= requests * max_new) {
     PagedAttnParams f = p;
     f.most_rows = (int)small;
     if (int rc = attn_paged_few(f, small, (int)head_dim, dtype, st)) return rc;
