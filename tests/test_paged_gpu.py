@@ -454,3 +454,58 @@ def test_rows_before_the_first_request(mt, dtype, max_new):
     got = O.numpy()
     assert (got[:5] == 7).all() and (np.abs(got[5:] - want) <= tol).all() and len(got) == n + 5
     no_device_flag(mt)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+def test_offsets_beyond_32_bits(mt, dtype):
+    """A pool of 70000 pages (9 or 18 GB with its values): its last pages lie more than 2^31 elements from its start."""
+    F, pages, Hk, page, D = mt.fused_ops, 70000, 4, 64, 128
+    big = [mt.DeviceArray.empty((pages, Hk, page, D), dtype) for _ in range(2)]
+    small = [mt.DeviceArray.zeros((8, Hk, page, D), dtype) for _ in range(2)]
+    r = np.random.default_rng(0)
+    lens, fresh = [150, 200], [1, 60]
+    n = sum(lens)
+    tables = np.array([[3, 1, 6, -1], [0, 7, 2, 5]], np.int32)
+    pos = np.concatenate([np.arange(k) for k in lens])
+    row = np.repeat([0, 1], lens)
+    slot = tables[row, pos // page] * page + pos % page
+    k, v = (dev(mt, r.standard_normal((n, Hk, D)), dtype) for _ in range(2))
+    q = dev(mt, r.standard_normal((sum(fresh), 8, D)), dtype)
+    F.fused_paged_append(k, v, *small, i32(mt, slot))
+    F.fused_paged_append(k, v, *big, i32(mt, slot + (pages - 8) * page))
+    for max_new in (1, 60):
+        ask = lambda pools, t: F.fused_paged_attention(q, *pools, i32(mt, t), i32(mt, [0, 1, 61]), i32(mt, lens), max_new=max_new).numpy()
+        assert np.array_equal(ask(big, np.where(tables >= 0, tables + pages - 8, -1)), ask(small, tables))
+    no_device_flag(mt)
+
+
+def bits(mt):
+    """Outputs of every kernel, on whatever stream and with whatever overlap is set."""
+    return [Step(batch, 4, 2, D, 16, dtype).run(mt, max_new=m) for dtype in DTYPES for D in (64, 128)
+            for batch, m in (([(3000, 1), (150, 1)], 1), (MIXED, 150), ([(40, 1), (9, 1)], 1))]
+
+
+def test_without_overlap_and_on_another_stream(mt, tmp_path):
+    """Kernels that start before their predecessor has ended read nothing that it writes: the same bits with the overlap
+    off (MT_PDL=0, read once per process), and on a stream of the caller's."""
+    import os
+    import subprocess
+    import sys
+    from mytorch_b200 import _lib, array
+    want = bits(mt)
+    code = f"import mytorch_b200 as mt, numpy as np, tests.test_paged_gpu as t; np.savez({str(tmp_path / 'x.npz')!r}, *t.bits(mt))"
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    child = subprocess.run([sys.executable, "-c", code], cwd=root, env=dict(os.environ, MT_PDL="0"), capture_output=True, text=True, timeout=300)
+    assert child.returncode == 0, child.stderr[-2000:]
+    with np.load(tmp_path / "x.npz") as z:
+        assert all(np.array_equal(z[f"arr_{i}"], w) for i, w in enumerate(want))
+    mine, before = ctypes.c_void_p(), array.stream()
+    array.synchronize()
+    _lib.stream_create(ctypes.byref(mine))
+    array.set_stream(mine)
+    try:
+        assert all(np.array_equal(a, b) for a, b in zip(bits(mt), want))
+        array.synchronize()
+    finally:
+        array.set_stream(before)
+    _lib.stream_destroy(mine)
