@@ -55,13 +55,16 @@ class PagedKVCache:
             raise RuntimeError(f"request {int(after.argmax())} would hold {int(after.max())} tokens of at most {self.max_len}")
         if self.pages_used(after) > self.shape[1]:
             raise RuntimeError(f"{self.pages_used(after)} pages are needed and {self.shape[1]} exist: release a request first")
-        if self._fresh is None or not np.array_equal(self._fresh, counts):      # a decoding step asks for the same as the one before
-            self._fresh, self._fresh_dev = counts, DeviceArray.from_numpy(counts, "int32")
+        # A decoding step asks for the same as the one before. How many counts were given belongs to it: there are as many last rows.
+        if self._fresh is None or not np.array_equal(self._fresh, fresh):
+            self._fresh = None                                   # until everything below is made
             n = int(counts.sum())
+            self._fresh_dev = DeviceArray.from_numpy(counts, "int32")
             self.starts = DeviceArray.empty((len(counts) + 1,), "int32")
             self.position, self.slot = DeviceArray.empty((n,), "int32"), DeviceArray.empty((n,), "int32")
             self.last_rows = DeviceArray.from_numpy(np.maximum(np.cumsum(counts)[:max(1, len(fresh))] - 1, 0), "int32")
             self.max_new, self.rows = int(counts.max()), n
+            self._fresh = fresh.copy()
         K.fused_paged_tables(self._held, self._fresh_dev, self.tables, self.free_pages, self._n_free, self.page_size,
                              out=(self.starts, self._kv_len, self.position, self.slot, self._next_free))
         self._held, self._kv_len = self._kv_len, self._held

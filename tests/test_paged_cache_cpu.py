@@ -1,0 +1,102 @@
+"""The host side of the paged cache: what begin(), update(), release() and generate() announce and refuse. Device arrays
+are NumPy arrays here and the library's calls are done by hand, so these run without a GPU."""
+import numpy as np
+import pytest
+
+
+class Array:
+    """A device array's shape, type and contents on the host."""
+
+    def __init__(self, a):
+        self.a = np.asarray(a)
+
+    shape = property(lambda self: self.a.shape)
+    dtype = property(lambda self: str(self.a.dtype))
+    size = property(lambda self: self.a.size)
+
+    @classmethod
+    def empty(cls, shape, dtype="float32"):
+        return cls(np.zeros(shape, dtype))
+
+    zeros = empty
+
+    @classmethod
+    def from_numpy(cls, a, dtype=None):
+        return cls(np.array(a, dtype))
+
+    def numpy(self):
+        return self.a.copy()
+
+    def reshape(self, *shape):
+        return Array(self.a.reshape(*shape))
+
+    def rows(self, a, b):
+        return Array(self.a[a:b])
+
+
+def tables(held, fresh, table, free, n_free, page, out):
+    """fused_paged_tables, one page after the other."""
+    starts, kv_len, position, slot, left = (o.a for o in out)
+    n = int(n_free.a[0])
+    starts[0] = 0
+    for r, (h, f) in enumerate(zip(held.a, fresh.a)):
+        for at in range(-(-h // page), -(-(h + f) // page)):
+            n -= 1
+            table.a[r, at] = free.a[n]
+        starts[r + 1], kv_len[r] = starts[r] + f, h + f
+        j = np.arange(h, h + f)
+        position[starts[r]:starts[r + 1]] = j
+        slot[starts[r]:starts[r + 1]] = table.a[r, j // page] * page + j % page
+    left[0] = n
+
+
+def release(done, table, kv_len, free, n_free, page):
+    for r in np.flatnonzero(done.a):
+        for at in range(-(-kv_len.a[r] // page)):
+            free.a[n_free.a[0]] = table.a[r, at]
+            n_free.a[0] += 1
+            table.a[r, at] = -1
+        kv_len.a[r] = 0
+
+
+def append(k, v, k_pages, v_pages, slot, strides=None):
+    page = k_pages.shape[2]
+    for i, s in enumerate(slot.a):
+        k_pages.a[s // page, :, s % page], v_pages.a[s // page, :, s % page] = k.a[i], v.a[i]
+
+
+@pytest.fixture()
+def paged(monkeypatch):
+    from mytorch_b200 import paged
+    monkeypatch.setattr(paged, "DeviceArray", Array)
+    monkeypatch.setattr(paged.K, "fused_paged_tables", tables)
+    monkeypatch.setattr(paged.K, "fused_paged_release", release)
+    monkeypatch.setattr(paged.K, "fused_paged_append", append)
+    return paged
+
+
+def a_cache(paged, **how):
+    return paged.PagedKVCache(**{**dict(num_pages=12, page_size=4, num_heads=1, head_dim=64, num_layers=2, max_requests=3, max_len=16), **how})
+
+
+def fill(cache, value=1.0):
+    """The step's rows of every layer."""
+    for layer in range(cache.shape[0]):
+        cache.update(*(Array(np.full((cache.rows, 1, 64), value, np.float32)) for _ in range(2)), layer)
+
+
+def step(cache, fresh):
+    cache.begin(fresh)
+    fill(cache)
+    return cache
+
+
+def test_one_row_of_logits_for_every_count_given(paged):
+    """Counts that are filled up with zeros to the same step still ask for another number of rows."""
+    cache = a_cache(paged)
+    assert list(step(cache, [1, 1]).last_rows.a) == [0, 1]
+    assert len(step(cache, [1, 1, 0]).last_rows.a) == 3
+    assert len(step(cache, [1, 1]).last_rows.a) == 2
+    assert len(step(cache, [1]).last_rows.a) == 1
+    assert len(step(cache, [1, 0]).last_rows.a) == 2
+    assert list(cache.lengths) == [5, 3, 0] and list(cache.kv_len.a) == [5, 3, 0]
