@@ -270,8 +270,8 @@ class GPT2(nn.Module):
         return out
 
     def _paged(self, input_ids, cache):
-        """Logits [requests, 1, V] behind each request's last new token; input_ids [1, tokens] as announced by
-        cache.begin(). Position rows are gathered by position."""
+        """Logits [requests, 1, V] behind each request's last new token, zeros where it has none; input_ids [1, tokens] as
+        announced by cache.begin(). Position rows are gathered by position."""
         cfg, e = self.config, self.embeddings
         if Tensor.build_graph_enabled() and any(p.requires_grad for p in self.parameters()):
             raise NotImplementedError("a paged cache holds no graph: run the forward under no_grad()")
@@ -283,7 +283,7 @@ class GPT2(nn.Module):
         for layer_idx, block in enumerate(self.blocks):
             x = block(x, cache=cache, layer_idx=layer_idx)
         last = Tensor(fused_ops.fused_embedding_forward(x.data.reshape(-1, cfg.embed_dim), cache.last_rows))
-        return self.lm_head(self.final_layer_norm(last)).data.reshape(cache.last_rows.size, 1, cfg.vocab_size)
+        return cache.clear_idle(self.lm_head(self.final_layer_norm(last)).data.reshape(cache.last_rows.size, 1, cfg.vocab_size))
 
     def forward(self, x, cache=None):
         """Logits; with a `Cache` (or a paged.PagedKVCache), (logits, cache) as in gpt2.py:352-374."""

@@ -258,8 +258,8 @@ class GPT(nn.Module):
         return out
 
     def _paged(self, input_ids, cache):
-        """Logits [requests, 1, V] behind each request's last new token; input_ids [1, tokens] as announced by
-        cache.begin(). Rotary rows are gathered by position."""
+        """Logits [requests, 1, V] behind each request's last new token, zeros where it has none; input_ids [1, tokens] as
+        announced by cache.begin(). Rotary rows are gathered by position."""
         cfg = self.config
         if Tensor.build_graph_enabled() and any(p.requires_grad for p in self.parameters()):
             raise NotImplementedError("a paged cache holds no graph: run the forward under no_grad()")
@@ -273,7 +273,7 @@ class GPT(nn.Module):
         if cfg.softcap and not self.training:
             arr = logits.data
             _lib.softcap(arr.ptr, arr.ptr, arr.size, float(cfg.softcap), arr.code, stream())
-        return logits.data.reshape(cache.last_rows.size, 1, cfg.vocab_size)
+        return cache.clear_idle(logits.data.reshape(cache.last_rows.size, 1, cfg.vocab_size))
 
     def forward(self, input_ids, target_ids=None, cache=None):
         if isinstance(cache, paged.PagedKVCache):

@@ -5,7 +5,7 @@ Both models' forward takes one as `cache`, with the new tokens of all requests p
 
     cache = PagedKVCache(num_pages=512, page_size=16, num_heads=kv_heads, head_dim=D, num_layers=L, max_requests=8, max_len=2048)
     cache.begin([5, 0, 9])                       # 5 new tokens for request 0, 9 for request 2
-    logits, cache = model(packed_ids, cache=cache)   # ids [1, 14] -> logits [3, 1, V] behind each request's last token
+    logits, cache = model(packed_ids, cache=cache)   # ids [1, 14] -> logits [3, 1, V] behind each request's last token, 0 for request 1
     cache.release([0])                           # request 0 is over; its pages are free again
 
 Tables, slots and positions are computed on the device (fused_ops.fused_paged_tables); the host keeps the
@@ -64,6 +64,7 @@ class PagedKVCache:
             self.position, self.slot = DeviceArray.empty((n,), "int32"), DeviceArray.empty((n,), "int32")
             self.last_rows = DeviceArray.from_numpy(np.maximum(np.cumsum(counts)[:max(1, len(fresh))] - 1, 0), "int32")
             self.max_new, self.rows = int(counts.max()), n
+            self._idle = np.flatnonzero(np.diff(np.r_[0, fresh == 0, 0])).reshape(-1, 2).tolist()     # [first, end) of requests without new tokens
             self._fresh = fresh.copy()
         K.fused_paged_tables(self._held, self._fresh_dev, self.tables, self.free_pages, self._n_free, self.page_size,
                              out=(self.starts, self._kv_len, self.position, self.slot, self._next_free))
@@ -93,6 +94,12 @@ class PagedKVCache:
         out = DeviceArray.empty(q.shape, q.dtype)                # begin()'s rows are exactly the requests' rows
         return K.fused_paged_attention(q, self._layer(self.k_pages, layer_idx), self._layer(self.v_pages, layer_idx), self.tables,
                                        self.starts, self._held, max_new=self.max_new, out=out, strides=strides)
+
+    def clear_idle(self, logits):
+        """Logits [requests, ...]: zeros for the requests that have no new token, whose last row is another request's."""
+        for first, end in self._idle:
+            logits.rows(first, end).zero_()
+        return logits
 
     def check(self, ids_shape, num_layers, num_heads, head_dim, max_positions):
         """Refuses a model or ids that this cache and step are not for."""

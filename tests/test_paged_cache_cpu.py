@@ -33,6 +33,9 @@ class Array:
     def rows(self, a, b):
         return Array(self.a[a:b])
 
+    def zero_(self):
+        self.a[...] = 0
+
 
 def tables(held, fresh, table, free, n_free, page, out):
     """fused_paged_tables, one page after the other."""
@@ -100,3 +103,11 @@ def test_one_row_of_logits_for_every_count_given(paged):
     assert len(step(cache, [1]).last_rows.a) == 1
     assert len(step(cache, [1, 0]).last_rows.a) == 2
     assert list(cache.lengths) == [5, 3, 0] and list(cache.kv_len.a) == [5, 3, 0]
+
+
+def test_requests_without_new_tokens_have_no_logits(paged):
+    cache = a_cache(paged, max_requests=6)
+    for fresh in ([5, 0, 3], [0, 1, 1], [1, 0, 0, 2, 0], [0, 0, 0, 0, 0, 1], [1, 1], [0, 1, 0]):
+        step(cache, fresh)
+        got = cache.clear_idle(Array(np.full((len(fresh), 1, 7), 3.0)))
+        assert (got.a[:, 0] == np.where(np.array(fresh)[:, None] > 0, 3.0, 0.0)).all(), fresh

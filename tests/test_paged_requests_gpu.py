@@ -1,0 +1,38 @@
+"""Requests over a paged cache at the edges of what a step may ask for, through both models."""
+import numpy as np
+import pytest
+
+from tests.test_infer_gpu import cache_of, models
+from tests.test_ops_gpu import DTYPES, TOL, close, no_device_flag
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def mt():
+    import mytorch_b200 as m
+    return m
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind,heads,kv_heads", [("gpt2", 2, 2), ("nanochat", 4, 2)])
+def test_idle_requests_and_lists_of_other_lengths(mt, dtype, kind, heads, kv_heads):
+    """A request without new tokens has zeros, wherever it stands; a list of counts with other zeros at its end asks for as many
+    rows as it has counts; the others have the logits of each request alone."""
+    model = models(mt, kind, dtype, heads, kv_heads, 64, False)
+    r = np.random.default_rng(11)
+    ids = [r.integers(0, 200, 30).astype(np.int32) for _ in range(4)]
+    cache, alone, at = mt.PagedKVCache(40, 16, kv_heads, 64, 2, 4, 160), [cache_of(mt, model, kind, 1) for _ in ids], [0] * 4
+    with mt.no_grad():
+        for fresh in ([5, 0, 9], [1, 0, 1], [1, 0, 1, 0], [0, 1, 1, 1], [0, 1, 1, 1], [1, 0], [1], [0, 0, 0, 1]):
+            new = [a[i:i + n] for a, i, n in zip(ids, at, fresh)]
+            logits = model(mt.Tensor(np.concatenate(new)[None]), cache=cache.begin(fresh))[0].numpy()
+            assert logits.shape[:2] == (len(fresh), 1)
+            for i, x in enumerate(new):
+                at[i] += len(x)
+                if len(x):
+                    want = model(mt.Tensor(x[None]), cache=alone[i])[0].numpy()[0, -1]
+                    close(logits[i, 0], want, 2 * TOL[dtype], f"request {i} of {fresh}")
+                else:
+                    assert (logits[i] == 0).all(), (i, fresh)
+    no_device_flag(mt)
