@@ -81,16 +81,22 @@ class PagedKVCache:
         self.lengths[done != 0] = 0
 
     def _layer(self, pools, layer_idx):
+        if not 0 <= layer_idx < self.shape[0]:
+            raise IndexError(f"layer {layer_idx} of {self.shape[0]}")
         return pools.rows(layer_idx, layer_idx + 1).reshape(self.shape[1:])
 
     def update(self, k, v, layer_idx, strides=None):
         """The step's new keys and values [rows, heads, head_dim] of one layer (`strides`: two Strides3 of a view)."""
+        if self.slot is None:
+            raise RuntimeError("no step was begun")
         if self.k_pages is None:
             self.k_pages, self.v_pages = (DeviceArray.zeros(self.shape, k.dtype) for _ in range(2))
         K.fused_paged_append(k, v, self._layer(self.k_pages, layer_idx), self._layer(self.v_pages, layer_idx), self.slot, strides)
 
     def attend(self, q, layer_idx, strides=None):
         """Causal attention of the step's rows q [rows, query heads, head_dim] over one layer's pages."""
+        if self.k_pages is None:
+            raise RuntimeError("no row was appended yet")
         out = DeviceArray.empty(q.shape, q.dtype)                # begin()'s rows are exactly the requests' rows
         return K.fused_paged_attention(q, self._layer(self.k_pages, layer_idx), self._layer(self.v_pages, layer_idx), self.tables,
                                        self.starts, self._held, max_new=self.max_new, out=out, strides=strides)

@@ -111,3 +111,24 @@ def test_requests_without_new_tokens_have_no_logits(paged):
         step(cache, fresh)
         got = cache.clear_idle(Array(np.full((len(fresh), 1, 7), 3.0)))
         assert (got.a[:, 0] == np.where(np.array(fresh)[:, None] > 0, 3.0, 0.0)).all(), fresh
+
+
+@pytest.mark.parametrize("layer", [2, -1, 5])
+def test_layers_that_the_cache_does_not_have(paged, layer, monkeypatch):
+    """Such a layer's pools would lie outside the memory of the cache: nothing is queued for it."""
+    cache = step(a_cache(paged), [3])
+    for name in ("fused_paged_append", "fused_paged_attention"):
+        monkeypatch.setattr(paged.K, name, lambda *a, **k: pytest.fail("reached the library"))
+    rows = Array(np.zeros((3, 1, 64), np.float32))
+    for call in (lambda: cache.update(rows, rows, layer), lambda: cache.attend(rows, layer)):
+        with pytest.raises(IndexError):
+            call()
+
+
+def test_calls_before_there_is_anything_to_work_on(paged):
+    cache, rows = a_cache(paged), Array(np.zeros((3, 1, 64), np.float32))
+    with pytest.raises(RuntimeError):
+        cache.update(rows, rows, 0)                              # no step was begun
+    cache.begin([3])
+    with pytest.raises(RuntimeError):
+        cache.attend(rows, 0)                                    # no row was ever appended
