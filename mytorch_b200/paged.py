@@ -97,6 +97,8 @@ class PagedKVCache:
         """Causal attention of the step's rows q [rows, query heads, head_dim] over one layer's pages."""
         if self.k_pages is None:
             raise RuntimeError("no row was appended yet")
+        if q.shape[0] != self.rows:
+            raise ValueError(f"begin() announced {self.rows} tokens, got queries of {q.shape[0]}")
         out = DeviceArray.empty(q.shape, q.dtype)                # begin()'s rows are exactly the requests' rows
         return K.fused_paged_attention(q, self._layer(self.k_pages, layer_idx), self._layer(self.v_pages, layer_idx), self.tables,
                                        self.starts, self._held, max_new=self.max_new, out=out, strides=strides)

@@ -132,3 +132,12 @@ def test_calls_before_there_is_anything_to_work_on(paged):
     cache.begin([3])
     with pytest.raises(RuntimeError):
         cache.attend(rows, 0)                                    # no row was ever appended
+
+
+@pytest.mark.parametrize("rows", [2, 4])
+def test_as_many_queries_as_the_step_has_rows(paged, rows, monkeypatch):
+    """More would leave rows of the result as they were allocated, fewer would leave out rows of requests."""
+    cache = step(a_cache(paged), [2, 1])
+    monkeypatch.setattr(paged.K, "fused_paged_attention", lambda *a, **k: pytest.fail("reached the library"))
+    with pytest.raises(ValueError):
+        cache.attend(Array(np.zeros((rows, 1, 64), np.float32)), 0)
