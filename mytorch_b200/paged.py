@@ -89,9 +89,9 @@ class PagedKVCache:
         """The step's new keys and values [rows, heads, head_dim] of one layer (`strides`: two Strides3 of a view)."""
         if self.slot is None:
             raise RuntimeError("no step was begun")
-        if self.k_pages is None:
-            self.k_pages, self.v_pages = (DeviceArray.zeros(self.shape, k.dtype) for _ in range(2))
-        K.fused_paged_append(k, v, self._layer(self.k_pages, layer_idx), self._layer(self.v_pages, layer_idx), self.slot, strides)
+        pools = (self.k_pages, self.v_pages) if self.k_pages is not None else [DeviceArray.zeros(self.shape, k.dtype) for _ in range(2)]
+        K.fused_paged_append(k, v, *(self._layer(p, layer_idx) for p in pools), self.slot, strides)
+        self.k_pages, self.v_pages = pools                       # the first rows that are taken settle the type
 
     def attend(self, q, layer_idx, strides=None):
         """Causal attention of the step's rows q [rows, query heads, head_dim] over one layer's pages."""

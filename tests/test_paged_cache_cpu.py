@@ -141,3 +141,16 @@ def test_as_many_queries_as_the_step_has_rows(paged, rows, monkeypatch):
     monkeypatch.setattr(paged.K, "fused_paged_attention", lambda *a, **k: pytest.fail("reached the library"))
     with pytest.raises(ValueError):
         cache.attend(Array(np.zeros((rows, 1, 64), np.float32)), 0)
+
+
+def test_a_refused_first_update_leaves_no_pools_behind(paged, monkeypatch):
+    """The pools have the type of the first rows that are taken, not of some that were refused."""
+    def refuse(*a, **k):
+        raise TypeError
+    cache = a_cache(paged).begin([3])
+    with monkeypatch.context() as m:
+        m.setattr(paged.K, "fused_paged_append", refuse)
+        with pytest.raises(TypeError):
+            cache.update(*(Array(np.zeros((3, 1, 64), np.int32)) for _ in range(2)), 0)
+    fill(cache)
+    assert cache.k_pages.dtype == cache.v_pages.dtype == "float32"
