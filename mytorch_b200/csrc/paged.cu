@@ -248,10 +248,10 @@ int mt_paged_tables(const int32_t* held, const int32_t* fresh, int32_t* tables, 
   MT_REQUIRE(kv_len != held && kv_len != fresh && n_free_out != n_free, "paged_tables: kv_len and n_free_out need buffers of their own");
   int64_t blocks = (rows + kTabThreads - 1) / kTabThreads;
   blocks = blocks < 1 ? 1 : blocks > sm_count() ? sm_count() : blocks;
-  const size_t smem = 2 * requests * sizeof(int);
-  if (smem > 48 * 1024)
-    MT_CHECK_CUDA(cudaFuncSetAttribute(paged_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kMaxRequests * (int)sizeof(int)));
-  paged_tables_kernel<<<(unsigned)blocks, kTabThreads, smem, as_stream(stream)>>>(
+  // raised whatever the size: the 48 KB that need no asking hold the static shared memory (512 bytes) as well
+  static SmemLimit limit;
+  if (int rc = limit.raise((const void*)paged_tables_kernel, 2 * kMaxRequests * (int)sizeof(int))) return rc;
+  paged_tables_kernel<<<(unsigned)blocks, kTabThreads, 2 * requests * sizeof(int), as_stream(stream)>>>(
       held, fresh, tables, free_pages, n_free, starts, kv_len, position, slot, n_free_out, (int)requests, (int)width,
       FastDiv((uint32_t)page_size), list_len, rows, device_flag_ptr());
   MT_LAUNCH_CHECK();

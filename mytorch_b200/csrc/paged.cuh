@@ -1,6 +1,7 @@
 // The paged key/value cache: what its kernels share (see mytorch_b200.h for the layout).
 #pragma once
 #include "common.cuh"
+#include <atomic>
 
 namespace mt {
 
@@ -16,6 +17,19 @@ struct FastDiv {
     m = (uint32_t)((((1ull << s) - div) << 32) / div + 1);
   }
   __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(m, n) + n) >> s; }
+};
+
+// A kernel's limit on dynamic shared memory, raised once per device (racing first calls raise it twice, harmlessly).
+struct SmemLimit {
+  std::atomic<bool> done[16] = {};
+  int raise(const void* kern, int bytes) {
+    int dev = 0;
+    MT_CHECK_CUDA(cudaGetDevice(&dev));
+    if (dev >= 0 && dev < 16 && done[dev].load(std::memory_order_acquire)) return MT_OK;
+    MT_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (dev >= 0 && dev < 16) done[dev].store(true, std::memory_order_release);
+    return MT_OK;
+  }
 };
 
 struct PagedAttnParams {

@@ -7,7 +7,6 @@
 // and sum per row) that a second kernel joins in the order of the keys, so results do not depend on timing.
 #pragma once
 #include "paged.cuh"
-#include <atomic>
 
 namespace mt {
 
@@ -250,19 +249,6 @@ inline WorkPartials partials_in(void* buf, int blocks, int M, int D) {
   w.cuts = (WorkPos*)(w.ml + (size_t)blocks * 2 * M * 2);
   return w;
 }
-
-// A kernel's limit on dynamic shared memory, raised once per device (racing first calls raise it twice, harmlessly).
-struct SmemLimit {
-  std::atomic<bool> done[16] = {};
-  int raise(const void* kern, int bytes) {
-    int dev = 0;
-    MT_CHECK_CUDA(cudaGetDevice(&dev));
-    if (dev >= 0 && dev < 16 && done[dev].load(std::memory_order_acquire)) return MT_OK;
-    MT_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    if (dev >= 0 && dev < 16) done[dev].store(true, std::memory_order_release);
-    return MT_OK;
-  }
-};
 
 // The block whose share begins at blockIdx.x tells the joining kernel so, if there is one.
 __device__ __forceinline__ void publish_share(const WorkShare& s, const WorkPartials& w) {
