@@ -122,14 +122,15 @@ class PagedKVCache:
 
 def generate(model, prompts, max_new_tokens, pick, new_cache):
     """Prompts of different lengths, each followed by max_new_tokens tokens: [ids + tokens per prompt].
-    pick(logits) -> next token per request, int32 [requests] on the device; new_cache(requests, longest, tokens in all)."""
+    pick(logits) -> next token per request, int32 [requests] on the device; new_cache(requests, the longest one's rows, every one's rows)."""
     prompts = [np.asarray(p, np.int32).reshape(-1) for p in prompts]
     if any(len(p) == 0 for p in prompts):
         raise ValueError("every prompt needs a token")
     if max_new_tokens < 1 or not prompts:
         return prompts
     R = len(prompts)
-    cache = new_cache(R, max(len(p) for p in prompts) + max_new_tokens, [len(p) + max_new_tokens for p in prompts])
+    rows = [len(p) + max_new_tokens - 1 for p in prompts]        # the last token is drawn and not fed
+    cache = new_cache(R, max(rows), rows)
     feed, fresh, out = DeviceArray.from_numpy(np.concatenate(prompts), "int32"), [len(p) for p in prompts], []
     for i in range(max_new_tokens):
         logits = model(feed.reshape(1, -1), cache.begin(fresh))
@@ -165,7 +166,7 @@ def sampler(temperature, top_k, rng):
 
 def cache_for(num_layers, num_heads, head_dim, page_size=16):
     """new_cache for generate(): just the pages that the requests will need."""
-    def make(requests, longest, totals):
-        pages = sum(-(-n // page_size) for n in totals)
+    def make(requests, longest, rows):
+        pages = sum(-(-n // page_size) for n in rows)
         return PagedKVCache(pages, page_size, num_heads, head_dim, num_layers, requests, longest)
     return make

@@ -154,3 +154,22 @@ def test_a_refused_first_update_leaves_no_pools_behind(paged, monkeypatch):
             cache.update(*(Array(np.zeros((3, 1, 64), np.int32)) for _ in range(2)), 0)
     fill(cache)
     assert cache.k_pages.dtype == cache.v_pages.dtype == "float32"
+
+
+@pytest.mark.parametrize("lengths,new", [([3, 6], 3), ([8, 1, 4], 1), ([16, 15], 1), ([9, 1], 8)])
+def test_generate_asks_for_no_more_than_it_feeds(paged, lengths, new):
+    """The last token is drawn and never fed: a request holds one row less than its tokens."""
+    made = []
+
+    def new_cache(requests, longest, rows):
+        made.append(paged.cache_for(2, 1, 64, page_size=4)(requests, longest, rows))
+        return made[0]
+
+    def model(ids, cache):
+        cache.check(ids.shape, 2, 1, 64, 16)
+        fill(cache)
+        return Array(np.zeros((len(lengths), 1, 5), np.float32))
+    out = paged.generate(model, [np.arange(n) for n in lengths], new, lambda logits: Array(np.full(len(lengths), 9, np.int32)), new_cache)
+    assert [list(o) for o in out] == [list(range(n)) + [9] * new for n in lengths]
+    held = np.array(lengths) + new - 1
+    assert list(made[0].lengths) == list(held) and made[0].max_len == held.max() and made[0].shape[1] == made[0].pages_used()

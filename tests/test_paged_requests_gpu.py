@@ -36,3 +36,18 @@ def test_idle_requests_and_lists_of_other_lengths(mt, dtype, kind, heads, kv_hea
                 else:
                     assert (logits[i] == 0).all(), (i, fresh)
     no_device_flag(mt)
+
+
+@pytest.mark.parametrize("kind", ["gpt2", "nanochat"])
+@pytest.mark.parametrize("lengths,new", [((3, 120, 17), 41), ((160, 9), 1)])
+def test_generate_up_to_the_last_position(mt, kind, lengths, new):
+    """160 positions: as far as each prompt alone, and no further."""
+    model = models(mt, kind, "float32", 2, 2, 64, False)
+    r = np.random.default_rng(9)
+    prompts = [r.integers(0, 200, n).astype(np.int32) for n in lengths]
+    got = model.generate(prompts, new, temperature=0)
+    for p, g in zip(prompts, got):
+        assert np.array_equal(g, model.generate(p[None], new, temperature=0)[0])
+    with pytest.raises(ValueError):
+        model.generate(prompts, new + 1, temperature=0)
+    no_device_flag(mt)
