@@ -34,6 +34,8 @@ class PagedKVCache:
         self.starts = self.position = self.slot = None
         self.lengths = np.zeros(max_requests, np.int64)          # the host's copy of the lengths
         self._fresh, self._fresh_dev = None, None
+        # The step's layers without its rows; whether a forward of it began; whether requests went since it began.
+        self._missing, self._running, self._released = set(), False, False
 
     @property
     def kv_len(self):
@@ -44,7 +46,10 @@ class PagedKVCache:
         return int((-(-(self.lengths if lengths is None else lengths) // self.page_size)).sum())
 
     def begin(self, fresh):
-        """Starts a step with fresh[r] new tokens for request r (shorter lists are filled up with zeros)."""
+        """Starts a step with fresh[r] new tokens for request r (shorter lists are filled up with zeros). From here on they count as
+        held, so after a forward that was refused or failed it is run again, or the step taken back by cancel(), before the next begins."""
+        if self._running and self._missing:
+            raise RuntimeError(f"the step before is without its rows in {len(self._missing)} of {self.shape[0]} layers: run its forward, or cancel() it")
         counts = np.zeros(len(self.lengths), np.int64)
         fresh = np.asarray(fresh, np.int64).reshape(-1)
         if len(fresh) > len(counts) or (fresh < 0).any():
@@ -57,7 +62,7 @@ class PagedKVCache:
             raise RuntimeError(f"{self.pages_used(after)} pages are needed and {self.shape[1]} exist: release a request first")
         # A decoding step asks for the same as the one before. How many counts were given belongs to it: there are as many last rows.
         if self._fresh is None or not np.array_equal(self._fresh, fresh):
-            self._fresh = None                                   # until everything below is made
+            self._end()                                          # until everything below is made
             n = int(counts.sum())
             self._fresh_dev = DeviceArray.from_numpy(counts, "int32")
             self.starts = DeviceArray.empty((len(counts) + 1,), "int32")
@@ -71,12 +76,35 @@ class PagedKVCache:
         self._held, self._kv_len = self._kv_len, self._held
         self._n_free, self._next_free = self._next_free, self._n_free
         self.lengths = after
+        self._missing, self._running, self._released = set(range(self.shape[0]) if self.rows else ()), False, False
         return self
+
+    def cancel(self):
+        """Takes the step back whose rows are not in every layer yet: lengths and free pages are as before its begin()."""
+        if not self._missing or self.slot is None:
+            raise RuntimeError("there is no step to take back: none was begun, or its rows are in every layer")
+        if self._released:
+            raise RuntimeError("requests were released since this step began: it can no longer be taken back")
+        self._held, self._kv_len = self._kv_len, self._held
+        self._n_free, self._next_free = self._next_free, self._n_free
+        self.lengths[:len(self._fresh)] -= self._fresh
+        self._end()
+
+    def _end(self):
+        """Nothing of this step can be asked for any more."""
+        self.starts = self.position = self.slot = self._fresh = None
+        self._missing, self._running = set(), False
 
     def release(self, requests):
         """These requests are over: their pages are free and their places may be used by new ones."""
         done = np.zeros(len(self.lengths), np.int32)
         done[np.asarray(requests, np.int64).reshape(-1)] = 1
+        if self._missing:
+            if done[:len(self._fresh)][self._fresh > 0].any():   # with tokens in this step
+                if self._running:
+                    raise RuntimeError("a request cannot go while a forward brings tokens for it: run it to its end, or cancel() the step")
+                self._end()
+            self._released = True
         K.fused_paged_release(DeviceArray.from_numpy(done, "int32"), self.tables, self._held, self.free_pages, self._n_free, self.page_size)
         self.lengths[done != 0] = 0
 
@@ -92,11 +120,13 @@ class PagedKVCache:
         pools = (self.k_pages, self.v_pages) if self.k_pages is not None else [DeviceArray.zeros(self.shape, k.dtype) for _ in range(2)]
         K.fused_paged_append(k, v, *(self._layer(p, layer_idx) for p in pools), self.slot, strides)
         self.k_pages, self.v_pages = pools                       # the first rows that are taken settle the type
+        self._running = True
+        self._missing.discard(layer_idx)
 
     def attend(self, q, layer_idx, strides=None):
         """Causal attention of the step's rows q [rows, query heads, head_dim] over one layer's pages."""
-        if self.k_pages is None:
-            raise RuntimeError("no row was appended yet")
+        if self.k_pages is None or self.slot is None:
+            raise RuntimeError("no row of this step was appended yet")
         if q.shape[0] != self.rows:
             raise ValueError(f"begin() announced {self.rows} tokens, got queries of {q.shape[0]}")
         out = DeviceArray.empty(q.shape, q.dtype)                # begin()'s rows are exactly the requests' rows
@@ -110,7 +140,8 @@ class PagedKVCache:
         return logits
 
     def check(self, ids_shape, num_layers, num_heads, head_dim, max_positions):
-        """Refuses a model or ids that this cache and step are not for."""
+        """Refuses a model or ids that this cache and step are not for. The step's forward begins here."""
+        self._running = True
         if self.starts is None or tuple(ids_shape) != (1, self.rows) or self.rows == 0:
             raise ValueError(f"begin() announced {0 if self.starts is None else self.rows} tokens; ids of shape (1, that many) are expected, got {tuple(ids_shape)}")
         L, _, H, _, D = self.shape

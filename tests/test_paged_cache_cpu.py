@@ -173,3 +173,95 @@ def test_generate_asks_for_no_more_than_it_feeds(paged, lengths, new):
     assert [list(o) for o in out] == [list(range(n)) + [9] * new for n in lengths]
     held = np.array(lengths) + new - 1
     assert list(made[0].lengths) == list(held) and made[0].max_len == held.max() and made[0].shape[1] == made[0].pages_used()
+
+
+def same_state(a, b):
+    """What later steps depend on: lengths, free pages in order, and the tables' entries in use."""
+    assert list(a.lengths) == list(b.lengths) and list(a.kv_len.a) == list(b.kv_len.a)
+    n = a._n_free.a[0]
+    assert n == b._n_free.a[0] and list(a.free_pages.a[:n]) == list(b.free_pages.a[:n])
+    for r, held in enumerate(a.lengths):
+        used = -(-held // a.page_size)
+        assert list(a.tables.a[r, :used]) == list(b.tables.a[r, :used])
+
+
+def test_a_step_whose_rows_were_not_appended(paged):
+    """Its rows would count as held and be read as keys and values: the next step is refused until they are there, or taken back."""
+    cache, other = step(a_cache(paged), [3, 5]), step(a_cache(paged), [3, 5])
+    cache.begin([6, 2])
+    with pytest.raises(ValueError):
+        cache.check((1, 7), 2, 1, 64, 16)                        # a forward that was refused
+    for appended in range(2):                                    # none of the two layers, one of them
+        for fresh in ([6, 2], [1], [0]):
+            with pytest.raises(RuntimeError):
+                cache.begin(fresh)
+        cache.update(*(Array(np.ones((8, 1, 64), np.float32)) for _ in range(2)), appended)
+    cache.begin([1, 0, 4]).cancel()                              # both are there: the next one, which is taken back
+    same_state(cache, step(other, [6, 2]))
+    rows = Array(np.ones((5, 1, 64), np.float32))
+    with pytest.raises(RuntimeError):
+        cache.update(rows, rows, 0)                              # a step that was taken back has no slots
+    same_state(step(cache, [2, 1]), step(other, [2, 1]))
+    with pytest.raises(RuntimeError):
+        cache.cancel()                                           # its rows are there
+
+
+def test_a_step_taken_back_half_way(paged):
+    cache, other = step(a_cache(paged), [3, 5]), step(a_cache(paged), [3, 5])
+    cache.begin([9, 2])
+    cache.update(*(Array(np.ones((11, 1, 64), np.float32)) for _ in range(2)), 1)
+    cache.cancel()
+    same_state(cache, other)
+    for c in (cache, other):
+        step(c, [1, 7, 2])
+        c.release([1])
+        step(c, [4, 3])
+    same_state(cache, other)
+
+
+def test_steps_without_tokens_leave_nothing_open(paged):
+    cache = a_cache(paged)
+    cache.begin([0, 0]).begin([]).begin([1])
+    assert list(cache.lengths) == [1, 0, 0]
+
+
+def test_release_within_a_step(paged):
+    """Requests that a forward under way brings tokens for cannot go; after others went, the step can no longer be taken back."""
+    cache, other = step(a_cache(paged), [3, 5]), step(a_cache(paged), [3, 5])
+    cache.begin([0, 2])
+    cache.update(*(Array(np.ones((2, 1, 64), np.float32)) for _ in range(2)), 0)
+    with pytest.raises(RuntimeError):
+        cache.release([1])
+    assert list(cache.lengths) == [3, 7, 0]
+    cache.release([0])
+    with pytest.raises(RuntimeError):
+        cache.cancel()
+    fill(cache)
+    other = step(other, [0, 2])
+    other.release([0])
+    same_state(cache, other)
+    cache.release([1])
+    assert sorted(cache.free_pages.a) == list(range(12))
+
+
+def test_a_program_with_pools_of_its_own(paged):
+    """One that takes tables and slots from the cache and appends by itself: steps follow each other, requests go when they like; a
+    request that went in a step leaves no step behind that a forward could run."""
+    cache, other = a_cache(paged), a_cache(paged)
+    for fresh, over in (([3, 5], []), ([1, 1, 2], [1]), ([2, 4], [0, 2]), ([0, 1], [])):
+        cache.begin(fresh)
+        assert len(cache.slot.a) == sum(fresh)
+        step(other, fresh)
+        for c in (cache, other):
+            c.release(over)
+        same_state(cache, other)
+    cache.release([1])
+    rows = Array(np.zeros((1, 1, 64), np.float32))
+    with pytest.raises(RuntimeError):
+        cache.update(rows, rows, 0)
+    with pytest.raises(RuntimeError):
+        cache.attend(rows, 0)
+    with pytest.raises(ValueError):
+        cache.check((1, 1), 2, 1, 64, 16)
+    other.release([1])
+    same_state(step(cache, [2]), step(other, [2]))

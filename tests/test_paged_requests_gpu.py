@@ -51,3 +51,37 @@ def test_generate_up_to_the_last_position(mt, kind, lengths, new):
     with pytest.raises(ValueError):
         model.generate(prompts, new + 1, temperature=0)
     no_device_flag(mt)
+
+
+@pytest.mark.parametrize("kind", ["gpt2", "nanochat"])
+def test_a_step_whose_forward_was_refused(mt, kind):
+    """Its rows are in no layer: the next step is refused, and after the step was taken back, or run with the right ids, every
+    logit is what it is without the refusal."""
+    model = models(mt, kind, "float16", 2, 2, 64, False)
+    r = np.random.default_rng(5)
+    ids = r.integers(0, 200, (3, 60)).astype(np.int32)
+    steps = [[20, 7], [1, 16, 30], [1, 1, 1]]
+
+    def run(disturb):
+        cache, out, at = mt.PagedKVCache(12, 16, 2, 64, 2, 3, 60), [], [0] * 3
+        for n, fresh in enumerate(steps):
+            new = np.concatenate([a[i:i + m] for a, i, m in zip(ids, at, fresh)])[None]
+            at = [i + (fresh[k] if k < len(fresh) else 0) for k, i in enumerate(at)]
+            cache.begin(fresh)
+            if disturb:
+                with pytest.raises(ValueError):
+                    model(mt.Tensor(new[:, :-1]), cache=cache)
+                with pytest.raises(RuntimeError):
+                    cache.begin(fresh)
+                if n != 1:
+                    cache.cancel()
+                    assert np.array_equal(cache.kv_len.numpy(), cache.lengths)
+                    cache.begin([2]).cancel()                    # another step, taken back too
+                    cache.begin(fresh)
+            out.append(model(mt.Tensor(new), cache=cache)[0].numpy())
+            assert np.array_equal(cache.kv_len.numpy(), cache.lengths)
+        return out
+    with mt.no_grad():
+        for a, b in zip(run(True), run(False)):
+            assert np.array_equal(a, b)
+    no_device_flag(mt)
