@@ -16,6 +16,14 @@ from . import _lib, fused_ops as K
 from .array import DeviceArray, stream
 
 
+def _whole(what, values, kinds="iuf"):
+    """Whole numbers of any type as int64; anything else is refused rather than rounded."""
+    a = np.asarray(values).reshape(-1)
+    if a.size and (a.dtype.kind not in kinds or not (np.abs(a) < 2 ** 31).all() or (a != np.floor(a)).any()):
+        raise ValueError(f"{what} are whole numbers below 2^31, got {values}")
+    return a.astype(np.int64)
+
+
 class PagedKVCache:
     def __init__(self, num_pages, page_size, num_heads, head_dim, num_layers, max_requests, max_len):
         if min(num_pages, page_size, num_heads, num_layers, max_requests, max_len) < 1:
@@ -51,7 +59,7 @@ class PagedKVCache:
         if self._running and self._missing:
             raise RuntimeError(f"the step before is without its rows in {len(self._missing)} of {self.shape[0]} layers: run its forward, or cancel() it")
         counts = np.zeros(len(self.lengths), np.int64)
-        fresh = np.asarray(fresh, np.int64).reshape(-1)
+        fresh = _whole("counts of new tokens", fresh, "iufb")
         if len(fresh) > len(counts) or (fresh < 0).any():
             raise ValueError(f"a step takes up to {len(counts)} counts of new tokens, none negative; got {fresh.tolist()}")
         counts[:len(fresh)] = fresh
@@ -98,7 +106,10 @@ class PagedKVCache:
     def release(self, requests):
         """These requests are over: their pages are free and their places may be used by new ones."""
         done = np.zeros(len(self.lengths), np.int32)
-        done[np.asarray(requests, np.int64).reshape(-1)] = 1
+        places = _whole("requests", requests)
+        if ((places < 0) | (places >= len(done))).any():
+            raise IndexError(f"the requests are 0 to {len(done) - 1}, got {places.tolist()}")
+        done[places] = 1
         if self._missing:
             if done[:len(self._fresh)][self._fresh > 0].any():   # with tokens in this step
                 if self._running:

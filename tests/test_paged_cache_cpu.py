@@ -265,3 +265,24 @@ def test_a_program_with_pools_of_its_own(paged):
         cache.check((1, 1), 2, 1, 64, 16)
     other.release([1])
     same_state(step(cache, [2]), step(other, [2]))
+
+
+def test_places_and_counts_that_are_none(paged):
+    cache = step(a_cache(paged), [3, 5, 1])
+    for bad in ([-1], [0, -3], [3], -1, 3):
+        with pytest.raises(IndexError):
+            cache.release(bad)
+    for bad in ([1.5], [True, False, True], ["1"], [float("nan")]):
+        with pytest.raises(ValueError):
+            cache.release(bad)
+    for bad in ([5.9], [float("nan")], [float("inf")], [2.0, 0.5], ["2"], [2 ** 63]):
+        with pytest.raises(ValueError):
+            cache.begin(bad)
+    assert list(cache.lengths) == [3, 5, 1] and list(cache.kv_len.a) == [3, 5, 1]
+    step(cache, [2.0, 1.0])                                      # whole numbers, whatever their type
+    step(cache, np.array([1, 1], np.uint8))
+    step(cache, [True, False])
+    cache.release(())
+    cache.release(np.array([0.0, 2.0]))
+    cache.release(1)
+    assert list(cache.lengths) == [0, 0, 0] and sorted(cache.free_pages.a) == list(range(12))
