@@ -331,13 +331,14 @@ class GPT(nn.Module):
         if paged.is_ragged(input_ids):
             was_training = self.training
             self.eval()
-            with no_grad():
-                out = paged.generate(lambda ids, cache: self._paged(Tensor(ids), cache), input_ids, max_new_tokens,
-                                     paged.sampler(temperature, top_k, rng),
-                                     paged.cache_for(cfg.num_blocks, cfg.num_kv_heads, cfg.embed_dim // cfg.num_q_heads))
-            if was_training:
-                self.train()
-            return out
+            try:
+                with no_grad():
+                    return paged.generate(lambda ids, cache: self._paged(Tensor(ids), cache), input_ids, max_new_tokens,
+                                          paged.sampler(temperature, top_k, rng),
+                                          paged.cache_for(cfg.num_blocks, cfg.num_kv_heads, cfg.embed_dim // cfg.num_q_heads))
+            finally:
+                if was_training:
+                    self.train()
         ids = np.asarray(input_ids.numpy() if isinstance(input_ids, Tensor) else input_ids, dtype=np.int32)
         cache = KVCache(ids.shape[0], cfg.num_kv_heads, cfg.max_seq_len, cfg.embed_dim // cfg.num_q_heads, cfg.num_blocks)
         was_training = self.training

@@ -286,3 +286,15 @@ def test_places_and_counts_that_are_none(paged):
     cache.release(np.array([0.0, 2.0]))
     cache.release(1)
     assert list(cache.lengths) == [0, 0, 0] and sorted(cache.free_pages.a) == list(range(12))
+
+
+def test_a_refused_generate_leaves_the_model_as_it_was():
+    """Prompts of different lengths, one of them empty: the model trains on afterwards."""
+    from types import SimpleNamespace
+    from mytorch_b200.nanochat_gpt import GPT
+    model = SimpleNamespace(training=True, config=SimpleNamespace(num_blocks=2, num_kv_heads=1, embed_dim=64, num_q_heads=1))
+    model.eval = lambda: setattr(model, "training", False)
+    model.train = lambda: setattr(model, "training", True)
+    with pytest.raises(ValueError):
+        GPT.generate(model, [[1, 2], []], 3)
+    assert model.training
