@@ -380,7 +380,7 @@ int mt_kv_append(const void* k_new, const void* v_new, void* k_cache, void* v_ca
 /* ---- the paged key/value cache ---------------------------------------------
  * Requests of different lengths that come and go (no counterpart in the reference, whose Cache,
  * gpt2_trainer/gpt2.py:29-86, holds one length for a whole batch). A layer's keys and values live in
- * two pools of n_pages pages of page_size rows, addressed with strides {page, head, row} (the
+ * two pools of n_pages pages of page_size rows, addressed with strides {page, head, row} (none negative, the
  * head_dim stride is 1). Row j of request r is row j % page_size of page tables[r, j / page_size]
  * (tables int32 [requests, width]). The new tokens of a step are packed: request r has rows
  * [starts[r], starts[r+1]). Everything a step needs of the lengths is computed on the device, so
@@ -413,7 +413,7 @@ int mt_paged_append(const void* k_new, const void* v_new, void* k_pages, void* v
 /* Attention of every request's new rows over its pages: kv_len[r] counts the keys of request r, its new
  * ones (already appended) among them; the last new row sees all of them, the row before it one less, and
  * so on (softmax(scale q.k) v over the visible keys; query head h reads key/value head
- * h / (heads / kv_heads)). q and o are [rows, heads, head_dim] with strides {unused, head, row}; rows that
+ * h / (heads / kv_heads)). q and o are [rows, heads, head_dim] with strides {unused, head, row}, none negative; rows that
  * no request has are not written. A row that sees no key, or only scores of -inf, is 0; what a row does not see does not
  * reach it, not even as NaN. Keys on a page outside the pool are left out (status word). max_new: the most
  * new rows a request is expected to have, which only picks the kernel (right for any lengths).

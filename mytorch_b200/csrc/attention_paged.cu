@@ -21,6 +21,8 @@ int mt_attn_paged(const void* q, const void* k_pages, const void* v_pages, void*
   const int64_t unit = 16 / (int64_t)dtype_size(dtype);
   MT_REQUIRE(spages.b % unit == 0 && spages.h % unit == 0 && spages.s % unit == 0 && aligned16(k_pages) && aligned16(v_pages),
              "attn_paged: the rows of the pools must be 16-byte aligned");
+  MT_REQUIRE(sq.h >= 0 && sq.s >= 0 && so.h >= 0 && so.s >= 0 && spages.b >= 0 && spages.h >= 0 && spages.s >= 0,
+             "attn_paged: negative strides");      // an offset below 0 is a row that is not there
   MT_REQUIRE(o != q, "attn_paged: the output needs a buffer of its own");
   MT_REQUIRE(scale > 0.f && scale < 2e38f, "attn_paged: scale must be a positive finite number");
   if (requests == 0 || rows == 0) return MT_OK;

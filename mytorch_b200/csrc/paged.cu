@@ -279,6 +279,7 @@ int mt_paged_append(const void* k_new, const void* v_new, void* k_pages, void* v
   MT_REQUIRE(page_size >= 1 && page_size < (1ll << 30) && n_pages < (1ll << 31) && n_pages * page_size < (1ll << 31),
              "paged_append: a pool has to hold fewer than 2^31 rows");
   MT_REQUIRE(rows < (1ll << 31) && kv_heads < (1ll << 31) && head_dim < (1ll << 28), "paged_append: bad sizes");
+  MT_REQUIRE(spages.b >= 0 && spages.h >= 0 && spages.s >= 0, "paged_append: negative strides of the pools");
   if (rows == 0) return MT_OK;
   const int e = (int)dtype_size(dtype);
   auto whole = [&](mt_strides3 s) { return s.h * e % 16 == 0 && s.s * e % 16 == 0; };
