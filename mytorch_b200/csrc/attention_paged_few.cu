@@ -95,12 +95,12 @@ struct FewLoader {
       if (valid) { kt = it.k0; window = -1; }
     }
     if (!valid) return;
-    const int key0 = first_key(warp), key1 = min(key0 + Cfg::kRows, it.keys) - 1;
-    if (key1 < key0) return;                                     // no row of this warp's in the tile
-    const int a = (int)p.page.div((uint32_t)key0), b = (int)p.page.div((uint32_t)key1);
-    if (window >= 0 && b < window + 32) return;
+    const int key0 = first_key(warp), n = min(Cfg::kRows, it.keys - key0);
+    if (n <= 0) return;                                          // no row of this warp's in the tile
+    const int a = (int)p.page.div((uint32_t)key0), b = (int)p.page.div((uint32_t)(key0 + n - 1));
+    if (window >= 0 && b - window < 32) return;
     window = a;
-    page = a + lane < p.width ? p.tables[(int64_t)it.r * p.width + a + lane] : -1;
+    page = lane < p.width - a ? p.tables[(int64_t)it.r * p.width + a + lane] : -1;
   }
   __device__ __forceinline__ void start(const PagedAttnParams& p, const WorkShare& s, int warp, int lane) {
     iter.start(s);
@@ -264,7 +264,7 @@ paged_few_half_kernel(const __grid_constant__ PagedAttnParams p, const WorkParti
               for (int n = 0; n < NT; ++n) mma16<T>(s[i][n], a, qf[n][k][0], qf[n][k][1]);
             }
         }
-        const bool full = mask == (uint32_t)((1ull << Cfg::kRows) - 1) && key0 + Cfg::kRows <= first_lim;
+        const bool full = mask == (uint32_t)((1ull << Cfg::kRows) - 1) && key0 <= first_lim - Cfg::kRows;
         if (!full) {
 #pragma unroll
           for (int n = 0; n < NT; ++n)

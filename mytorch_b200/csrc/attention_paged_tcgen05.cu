@@ -61,7 +61,7 @@ template <int D> struct PtCfg {
 __device__ __forceinline__ int subtile_tiles(const PagedAttnParams& p, const WorkItem& it, int s) {
   if (it.rows <= 128 * s) return 0;
   const int64_t rows = min((int64_t)it.t * kPtM + 128 * (s + 1), (int64_t)it.x.n_new * p.group);
-  const int n = (visible_keys(it.x, (int)p.by_group.div((uint32_t)(rows - 1))) + kPtKT - 1) / kPtKT;
+  const int n = key_tiles<kPtKT>(visible_keys(it.x, (int)p.by_group.div((uint32_t)(rows - 1))));
   return max(0, min(n, it.k1) - it.k0);
 }
 
@@ -165,7 +165,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       if (n == 0) { --tn; continue; }                    // no key: the softmax warps write zeros
       const int32_t* table = p.tables + (int64_t)it.r * p.width;
       // This lane's page of a tile (its box's or its row's) and the first row there.
-      auto key_at = [&](int kt) { return kt * kPtKT + (box_rows > 0 ? box * box_rows : lw * 32 + lane); };
+      auto key_at = [&](int kt) { return (int)((uint32_t)kt * kPtKT + (box_rows > 0 ? box * box_rows : lw * 32 + lane)); };
       auto page_at = [&](int kt) {
         if (kt >= it.k0 + n || (box_rows > 0 && lane >= boxes)) return -1;
         const int key = key_at(kt);
@@ -399,7 +399,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         }
         volatile const uint32_t* mask = masks + ((tiles + i) & 15) * 4;
         const bool all = (mask[0] & mask[1] & mask[2] & mask[3]) == 0xffffffffu;
-        if (!all || key0 + kPtKT > lim_min) {
+        if (!all || key0 > lim_min - kPtKT) {
           // What a row does not see becomes -inf where it lies, in pieces: rare tiles take longer, the others have no code for it.
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {

@@ -26,6 +26,10 @@ __device__ __forceinline__ int tile_keys(const PagedAttnParams& p, const PagedRe
   return visible_keys(x, (int)p.by_group.div((uint32_t)(rows - 1)));
 }
 
+// Key tiles that `keys` keys fill (up to 2^31 - 1 of them).
+template <int KT>
+__device__ __forceinline__ int key_tiles(int keys) { return (int)(((uint32_t)keys + KT - 1) / KT); }
+
 // Weight of the first T of nt tiles of one head, in key tiles: increasing, in closed form and free of
 // divisions (a block's first 2 us are this arithmetic, and every block does it). A tile's weight is FIXED for
 // queries in and output out, and the keys that its rows see; `slope` is what a tile sees more than the one before, M / (group * KT), in
@@ -152,7 +156,7 @@ __device__ __forceinline__ WorkShare find_share(const PagedAttnParams& p, int le
         if (weight_upto<KT, FIXED>(x, slope, mid, nt) <= cut) lo = mid; else hi = mid;
       }
       const int64_t begin = weight_upto<KT, FIXED>(x, slope, lo, nt), width = weight_upto<KT, FIXED>(x, slope, lo + 1, nt) - begin;
-      const int n = (tile_keys<M>(p, x, lo) + KT - 1) / KT;
+      const int n = key_tiles<KT>(tile_keys<M>(p, x, lo));
       const int kt = min(n - 1, (int)((float)(cut - begin) * (float)n / (float)width));
       const int snap = whole ? n / 2 : (int)fminf(1e9f, (float)total / (float)(NEAR * blocks));
       f.t = lo;
@@ -204,7 +208,7 @@ struct WorkIter {
     it.r = cur.r; it.hk = cur.hk; it.t = cur.t; it.x = x;
     it.rows = (int)min((int64_t)M, (int64_t)x.n_new * p.group - (int64_t)cur.t * M);
     it.keys = tile_keys<M>(p, x, cur.t);
-    it.n = (it.keys + KT - 1) / KT;
+    it.n = key_tiles<KT>(it.keys);
     it.k0 = cur.kt;
     it.k1 = same_item(cur, end) ? min(end.kt, it.n) : it.n;
     ++cur.t;

@@ -28,3 +28,40 @@ def child(code):
 def test_tables_as_a_process_first_call(requests):
     child("import numpy as np, mytorch_b200 as mt, tests.test_paged_gpu as t;"
           f"t.check_tables(mt, np.full({requests}, 15), np.full({requests}, 2), 16, 2, {requests}, {2 * requests})")
+
+
+@pytest.mark.parametrize("dtype,max_new", [("float16", 1), ("float16", 40), ("bfloat16", 40), ("float32", 1)])
+def test_the_longest_request_that_a_table_can_hold(mt, dtype, max_new):
+    """2^31 - 21 keys, the last ones in a tile that ends where 32-bit numbers do. Entries of the table may be equal: four pages over
+    and over, and a last one whose scores are 22 higher, so that its 11 keys weigh more than all others together.
+
+    Tolerance: an accumulator takes k sums one after the other over a block's share of the keys, each off by at most 2^-23 of it (the
+    tensor cores cut off, others round): tiles of 128 keys, a share of 2^24 / 444 of them with 4 sums each (few rows, half),
+    2^24 / 148 with 8 (many rows); 2^26 / 592 tiles of 32 keys with 8 (fp32). The weights' sum has no more, and 4 u covers the
+    roundings of weights and output. Scores are off by less than 2 (|q| |k| D 2^-24): 80 * 64 * 2^-24, far below."""
+    from tests.test_ops_gpu import dev, no_device_flag, rnd
+    from tests.test_paged_gpu import U, i32
+    D, page = 64, 16
+    width = 2 ** 27 - 1
+    keys = width * page - 5
+    r = np.random.default_rng(0)
+    k, v = (rnd(r.standard_normal((5, 1, page, D)), dtype) for _ in range(2))
+    q = rnd(r.standard_normal((1, 1, D)), dtype)
+    q[:, :, 0], k[:, :, :, 0] = 8, 0
+    k[4, :, :, 0] = 22                                           # a score of 22 = 8 * 22 / sqrt(D)
+    table = np.tile(np.arange(4, dtype=np.int32), 2 ** 25)[:width]
+    table[-1] = 4
+    got = mt.fused_ops.fused_paged_attention(dev(mt, q, dtype), dev(mt, k, dtype), dev(mt, v, dtype), i32(mt, table[None]), i32(mt, [0, 1]),
+                                             i32(mt, [keys]), max_new=max_new).numpy()[0, 0]
+    count = np.bincount(table, minlength=5).astype(np.float64).repeat(page).reshape(5, page)
+    count[4, page - 5:] = 0
+    s = np.einsum("d,pjd->pj", q[0, 0].astype(np.float64), k[:, 0].astype(np.float64)) / 8
+    p = count * np.exp(s - s.max())
+    p /= p.sum()
+    assert 0.3 < p[4].sum() < 0.99
+    want, A = np.einsum("pj,pjd->d", p, v[:, 0]), np.einsum("pj,pjd->d", p, np.abs(v[:, 0]))
+    sums = 2 ** 26 / 592 * 8 if dtype == "float32" else 2 ** 24 / 444 * 4 if max_new == 1 else 2 ** 24 / 148 * 8
+    allowed = (2 * sums * 2.0 ** -23 + 4 * U[dtype]) * A
+    print(dtype, max_new, "error", np.abs(got - want).max(), "of", np.abs(want).max(), "allowed", allowed.min(), "last page", p[4].sum())
+    assert (np.abs(got - want) <= allowed).all()
+    no_device_flag(mt)
