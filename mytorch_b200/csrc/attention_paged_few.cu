@@ -553,6 +553,9 @@ static int launch_few_rows(const PagedAttnParams& p, int64_t rows, cudaStream_t 
     // 19.2) and gain 7 % where bandwidth does (20 rows, 64 requests: 43.0 against 46.1).
     return launch_few<T, D, 16>(p, st);
   } else {
+    // Shares are weighed in 64 bits: tiles^2 / 2 * 2^11 M / group, which passes them between 2^27 and 2^28 rows of a request
+    // where M group <= 4.
+    if ((int64_t)p.rows * p.group >= 1 << 27) return launch_few<T, D, 8>(p, st);
     if (rows <= 1) return launch_few<T, D, 1>(p, st);
     if (rows <= 2) return launch_few<T, D, 2>(p, st);
     if (rows <= 4) return launch_few<T, D, 4>(p, st);

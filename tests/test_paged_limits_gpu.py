@@ -65,3 +65,23 @@ def test_the_longest_request_that_a_table_can_hold(mt, dtype, max_new):
     print(dtype, max_new, "error", np.abs(got - want).max(), "of", np.abs(want).max(), "allowed", allowed.min(), "last page", p[4].sum())
     assert (np.abs(got - want) <= allowed).all()
     no_device_flag(mt)
+
+
+def test_the_most_rows_of_one_request(mt):
+    """2^27 + 2^20 rows where a token was expected, in fp32: shares of them, weighed row by row, pass 64 bits. The last row sees
+    the one key there is, all others see none. (All rows read one query; the output takes 35 GB.)"""
+    torch = pytest.importorskip("torch")
+    from mytorch_b200 import _lib
+    from mytorch_b200.array import stream, synchronize
+    rows, D = 2 ** 27 + 2 ** 20, 64
+    out = torch.full((rows, D), float("nan"), device="cuda")
+    pools = torch.arange(2 * 16 * D, device="cuda", dtype=torch.float32).view(2, 1, 16, D)
+    ints = [torch.tensor(a, device="cuda", dtype=torch.int32) for a in ([[1, -1]], [0, rows], [1])]
+    torch.cuda.synchronize()
+    S = _lib.Strides3
+    _lib.attn_paged(pools.data_ptr(), pools.data_ptr(), pools.data_ptr(), out.data_ptr(), S(0, D, 0), S(16 * D, 16 * D, D), S(0, D, D),
+                    *[a.data_ptr() for a in ints], 1, 2, rows, 1, 1, 1, D, 16, 2, 0.125, _lib.F32, stream())
+    synchronize()
+    assert torch.equal(out[-1], pools[1, 0, 0])
+    step = 1 << 22
+    assert all(not out[a:min(a + step, rows - 1)].any() for a in range(0, rows, step))
