@@ -42,7 +42,7 @@ int mt_device_count(int* count);
 int mt_set_device(int device);
 int mt_get_device(int* device);
 int mt_device_sm_count(int* count);
-int mt_malloc(void** ptr, size_t bytes, void* stream);      /* stream-ordered, pooled */
+int mt_malloc(void** ptr, size_t bytes, void* stream);      /* stream-ordered, from the device's default pool, which then keeps what is freed */
 int mt_free(void* ptr, void* stream);
 int mt_host_alloc(void** ptr, size_t bytes);                /* pinned host memory */
 int mt_host_free(void* ptr);
@@ -417,7 +417,8 @@ int mt_paged_append(const void* k_new, const void* v_new, void* k_pages, void* v
  * no request has are not written. A row that sees no key, or only scores of -inf, is 0; what a row does not see does not
  * reach it, not even as NaN. Keys on a page outside the pool are left out (status word). max_new: the most
  * new rows a request is expected to have, which only picks the kernel (right for any lengths).
- * head_dim 64 or 128; page strides and pools 16-byte aligned; scale positive; o and q do not overlap.
+ * head_dim 64 or 128; page strides and pools 16-byte aligned; scale positive; o and q do not overlap. Scratch (up to 40 MB)
+ * comes from a pool of the library's own, which keeps what is freed.
  * (As everywhere here, the first call on a device goes before a capture.) */
 int mt_attn_paged(const void* q, const void* k_pages, const void* v_pages, void* o, mt_strides3 sq, mt_strides3 spages,
                   mt_strides3 so, const int32_t* tables, const int32_t* starts, const int32_t* kv_len,

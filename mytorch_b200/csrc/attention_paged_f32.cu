@@ -213,7 +213,7 @@ static int launch_paged_f32(const PagedAttnParams& p, cudaStream_t st) {
   static SmemLimit limit;
   if (int rc = limit.raise((const void*)kern, Cfg::kSmem)) return rc;
   const int grid = 2 * sm_count();
-  TempBuf part(partial_bytes(grid, kPfM, D), st);
+  TempBuf part(partial_bytes(grid, kPfM, D), st, Scratch::kOwnPool);
   if (!part.ok()) return MT_ERR_CUDA;
   const WorkPartials w = partials_in(part.ptr, grid, kPfM, D);
   MT_CHECK_CUDA(launch_overlapped(kern, dim3((unsigned)grid), dim3(kPfThreads), Cfg::kSmem, st, p, w, 3, tile_slope<kPfM, Cfg::KT>(p.group)));

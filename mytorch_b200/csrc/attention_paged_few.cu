@@ -536,7 +536,7 @@ static int launch_few(const PagedAttnParams& p, cudaStream_t st) {
   // Tables that end within a few tiles: no item is cut then, and there is nothing to join (a second launch costs 3 us, as
   // much as six tiles one after the other).
   const int whole = (int64_t)p.width * p.page.d <= 6 * Cfg::KT;
-  TempBuf part(whole ? 0 : partial_bytes(grid, M, D), st);
+  TempBuf part(whole ? 0 : partial_bytes(grid, M, D), st, Scratch::kOwnPool);
   if (!part.ok()) return MT_ERR_CUDA;
   const WorkPartials w = whole ? WorkPartials{} : partials_in(part.ptr, grid, M, D);
   MT_CHECK_CUDA(launch_overlapped(kern, dim3((unsigned)grid), dim3(kFewWarps * 32), Cfg::kSmem, st, p, w, 3, tile_slope<M, Cfg::KT>(p.group), whole));

@@ -582,7 +582,7 @@ static int launch_paged_tc(const PagedAttnParams& p, cudaStream_t st) {
   static SmemLimit limit;
   if (int rc = limit.raise((const void*)kern, Cfg::kSmem)) return rc;
   const int grid = sm_count();
-  TempBuf part(partial_bytes(grid, kPtM, D), st);
+  TempBuf part(partial_bytes(grid, kPtM, D), st, Scratch::kOwnPool);
   if (!part.ok()) return MT_ERR_CUDA;
   const WorkPartials w = partials_in(part.ptr, grid, kPtM, D);
   auto vec = [](const void* x, mt_strides3 s) { return aligned16(x) && s.h % 8 == 0 && s.s % 8 == 0; };

@@ -37,6 +37,7 @@ static constexpr int kMaxDev = 16;
 static int* g_flag[kMaxDev] = {nullptr};
 static int g_sms[kMaxDev] = {0};
 static bool g_pool_ready[kMaxDev] = {false};
+static cudaMemPool_t g_scratch[kMaxDev] = {nullptr};
 static std::mutex g_mu;
 
 int* device_flag_ptr() {
@@ -63,18 +64,28 @@ int sm_count() {
   return g_sms[dev];
 }
 
-// The device's pool keeps what is freed: without that every allocation after a synchronisation maps
-// memory anew (120 us).
-int ensure_pool() {
+// A pool of the library's own on the current device, which keeps what is freed: with the default one, where nobody
+// asked for that, every allocation after a synchronisation maps memory anew (120 us).
+int scratch_pool(cudaMemPool_t* pool) {
   int dev = 0;
   MT_CHECK_CUDA(cudaGetDevice(&dev));
-  if (dev < kMaxDev && !g_pool_ready[dev]) {
-    cudaMemPool_t pool;
-    MT_CHECK_CUDA(cudaDeviceGetDefaultMemPool(&pool, dev));
-    uint64_t thr = UINT64_MAX;  // keep freed blocks cached in the pool
-    MT_CHECK_CUDA(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &thr));
-    g_pool_ready[dev] = true;
+  MT_REQUIRE(dev < kMaxDev, "scratch: device %d of at most %d", dev, kMaxDev);
+  std::lock_guard<std::mutex> lk(g_mu);
+  if (!g_scratch[dev]) {
+    cudaMemPoolProps props = {};
+    props.allocType = cudaMemAllocationTypePinned;
+    props.location.type = cudaMemLocationTypeDevice;
+    props.location.id = dev;
+    cudaMemPool_t made;
+    MT_CHECK_CUDA(cudaMemPoolCreate(&made, &props));
+    uint64_t thr = UINT64_MAX;
+    if (cudaError_t e = cudaMemPoolSetAttribute(made, cudaMemPoolAttrReleaseThreshold, &thr)) {
+      cudaMemPoolDestroy(made);
+      MT_CHECK_CUDA(e);
+    }
+    g_scratch[dev] = made;
   }
+  *pool = g_scratch[dev];
   return MT_OK;
 }
 
@@ -134,6 +145,19 @@ int mt_device_count(int* count) {
 int mt_set_device(int device) { MT_CHECK_CUDA(cudaSetDevice(device)); return MT_OK; }
 int mt_get_device(int* device) { MT_CHECK_CUDA(cudaGetDevice(device)); return MT_OK; }
 int mt_device_sm_count(int* count) { *count = sm_count(); return MT_OK; }
+
+static int ensure_pool() {
+  int dev = 0;
+  MT_CHECK_CUDA(cudaGetDevice(&dev));
+  if (dev < kMaxDev && !g_pool_ready[dev]) {
+    cudaMemPool_t pool;
+    MT_CHECK_CUDA(cudaDeviceGetDefaultMemPool(&pool, dev));
+    uint64_t thr = UINT64_MAX;  // keep freed blocks cached in the pool
+    MT_CHECK_CUDA(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &thr));
+    g_pool_ready[dev] = true;
+  }
+  return MT_OK;
+}
 
 int mt_malloc(void** ptr, size_t bytes, void* stream) {
   *ptr = nullptr;

@@ -6,16 +6,18 @@
 #include "common.cuh"
 
 namespace mt {
-int ensure_pool();   // the current device's pool keeps what is freed
+int scratch_pool(cudaMemPool_t* pool);   // the library's own on the current device, which keeps what is freed
+enum class Scratch { kDevicePool, kOwnPool };
 
 struct TempBuf {
   void* ptr = nullptr;
   cudaStream_t st;
   bool ok_ = true;
-  TempBuf(size_t bytes, cudaStream_t s) : st(s) {
+  TempBuf(size_t bytes, cudaStream_t s, Scratch from = Scratch::kDevicePool) : st(s) {
     if (bytes == 0) return;
-    if (ensure_pool() != MT_OK) { ok_ = false; return; }
-    cudaError_t e = cudaMallocAsync(&ptr, bytes, s);
+    cudaMemPool_t pool;
+    if (from == Scratch::kOwnPool && scratch_pool(&pool) != MT_OK) { ok_ = false; return; }
+    cudaError_t e = from == Scratch::kOwnPool ? cudaMallocFromPoolAsync(&ptr, bytes, pool, s) : cudaMallocAsync(&ptr, bytes, s);
     if (e != cudaSuccess) {
       set_error("scratch allocation of %zu bytes failed: %s", bytes, cudaGetErrorString(e));
       ok_ = false;

@@ -85,3 +85,38 @@ def test_the_most_rows_of_one_request(mt):
     assert torch.equal(out[-1], pools[1, 0, 0])
     step = 1 << 22
     assert all(not out[a:min(a + step, rows - 1)].any() for a in range(0, rows, step))
+
+
+SCRATCH = """
+import ctypes, torch
+from mytorch_b200 import _lib, array
+cu = ctypes.CDLL("libcuda.so.1")
+def kept():
+    pool, n = ctypes.c_void_p(), ctypes.c_uint64()
+    assert cu.cuDeviceGetDefaultMemPool(ctypes.byref(pool), 0) == 0
+    assert cu.cuMemPoolGetAttribute(pool, 4, ctypes.byref(n)) == 0          # the release threshold
+    return n.value
+x = torch.ones(10000, device="cuda")
+out = torch.zeros(1, device="cuda")
+torch.cuda.synchronize()
+print(kept())
+_lib.sum_f32(x.data_ptr(), _lib.F32, x.numel(), out.data_ptr(), array.stream())
+print(kept())
+q, o, pools = (torch.zeros(s, device="cuda", dtype=torch.float16) for s in ((40, 2, 64), (40, 2, 64), (100, 2, 16, 64)))
+ints = [torch.tensor(a, device="cuda", dtype=torch.int32) for a in ([list(range(100))], [0, 40], [1600])]
+torch.cuda.synchronize()
+S = _lib.Strides3
+for max_new in (1, 40):
+    _lib.attn_paged(q.data_ptr(), pools.data_ptr(), pools.data_ptr(), o.data_ptr(), S(0, 64, 128), S(2048, 1024, 64), S(0, 64, 128),
+                    *[a.data_ptr() for a in ints], 1, 100, 40, max_new, 2, 2, 64, 16, 100, 0.125, _lib.F16, array.stream())
+    print(kept())
+array.synchronize()
+array.DeviceArray.empty((4,), "float32")
+print(kept())
+"""
+
+
+def test_scratch_leaves_the_process_memory_pool_alone():
+    """A program with buffers of its own keeps its device's default pool as it set it, whatever scratch the calls take; mt_malloc,
+    which allocates from that pool, has it keep what is freed."""
+    assert [int(n) for n in child(SCRATCH).split()] == [0, 0, 0, 0, 2 ** 64 - 1]
