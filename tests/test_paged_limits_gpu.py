@@ -120,3 +120,14 @@ def test_scratch_leaves_the_process_memory_pool_alone():
     """A program with buffers of its own keeps its device's default pool as it set it, whatever scratch the calls take; mt_malloc,
     which allocates from that pool, has it keep what is freed."""
     assert [int(n) for n in child(SCRATCH).split()] == [0, 0, 0, 0, 2 ** 64 - 1]
+
+
+# Groups of query heads that fill a box of queries but none of outputs (64, 128), and that pass a tile of 128 rows or an item of 256.
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("heads,kv_heads,D", [(64, 1, 64), (128, 2, 128), (128, 1, 64), (160, 1, 128), (320, 1, 64)])
+def test_many_query_heads_for_one_of_the_cache(mt, dtype, heads, kv_heads, D):
+    from tests.test_paged_gpu import Step, no_device_flag
+    for batch in ([(1, 1), (129, 1), (300, 1)], [(40, 3), (1, 1), (0, 0), (150, 9), (5, 5), (64, 0), (257, 2)]):
+        Step(batch, heads, kv_heads, D, 16, dtype).check(mt, max_new=max(m for _, m in batch))
+    Step([(70, 6), (33, 2)], heads, kv_heads, D, 7, dtype, pad=0).check(mt)
+    no_device_flag(mt)
