@@ -131,3 +131,32 @@ def test_many_query_heads_for_one_of_the_cache(mt, dtype, heads, kv_heads, D):
         Step(batch, heads, kv_heads, D, 16, dtype).check(mt, max_new=max(m for _, m in batch))
     Step([(70, 6), (33, 2)], heads, kv_heads, D, 7, dtype, pad=0).check(mt)
     no_device_flag(mt)
+
+
+def test_nan_at_the_start_of_a_long_cache(mt):
+    """A value that is NaN makes 256 rows of 140000 keys be computed again one by one, for 2.6 s, beside 295 requests that are finite: longer
+    than any wait within the kernel may last, so nothing may wait for it, and no row is lost: the others have the bits that they have
+    without it. The same rows' other columns, two ways: sums of fp16 weights (off by 2^-11) against fp32 ones, both of 140000 terms
+    in fp32 (140008 * 2^-24 of sum_j p_j |v_j| < 1 at most, in output and weights' sum), rounded once."""
+    from tests.test_ops_gpu import dev
+    from tests.test_paged_gpu import device_flag, i32
+    N, D, page, R, new = 140000, 64, 128, 296, 256
+    n = -(-N // page)
+    r = np.random.default_rng(0)
+    k, v = (r.standard_normal((n + 1, 1, page, D)).astype(np.float16) for _ in range(2))
+    k[n], v[n] = k[0], v[0]
+    v[n, 0, 3, 5] = np.nan
+    Q, K, V = (dev(mt, a, "float16") for a in (r.standard_normal((R * new, 1, D)), k, v))
+    tables = np.tile(np.arange(n), (R, 1))
+
+    def ask():
+        return mt.fused_ops.fused_paged_attention(Q, K, V, i32(mt, tables), i32(mt, np.arange(R + 1) * new), i32(mt, [N] * R),
+                                                  max_new=new).numpy()[:, 0]
+    clean = ask()
+    tables[0, 0] = n                                             # for request 0 alone
+    got = ask()
+    assert device_flag(mt) == 0 and np.isfinite(clean).all()
+    assert np.array_equal(got[new:], clean[new:])
+    assert np.isnan(got[:new, 5]).all()
+    a, b = (np.delete(x[:new], 5, 1).astype(np.float64) for x in (got, clean))
+    assert (np.abs(a - b) <= 3 * 2.0 ** -11 + 4 * (N + 8) * 2.0 ** -24).all()
