@@ -416,7 +416,9 @@ int mt_paged_append(const void* k_new, const void* v_new, void* k_pages, void* v
  * h / (heads / kv_heads)). q and o are [rows, heads, head_dim] with strides {unused, head, row}, none negative; rows that
  * no request has are not written. A row that sees no key, or only scores of -inf, is 0; what a row does not see does not
  * reach it, not even as NaN. Keys on a page outside the pool are left out (status word). max_new: the most
- * new rows a request is expected to have, which only picks the kernel (right for any lengths).
+ * new rows a request is expected to have. It picks the kernel, which is right for any lengths, and with it the rounding: for few
+ * rows (max_new * heads / kv_heads up to 32) the softmax's weights keep about fp32's precision, for many rows in half precision
+ * they are rounded to the type for the product, as the output is.
  * head_dim 64 or 128; page strides and pools 16-byte aligned; scale positive; o and q do not overlap. Scratch (up to 40 MB)
  * comes from a pool of the library's own, which keeps what is freed.
  * (As everywhere here, the first call on a device goes before a capture.) */

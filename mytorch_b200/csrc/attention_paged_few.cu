@@ -4,10 +4,10 @@
 // 4 D operations per query row). A block of four warps works on one item at a time: M rows (tokens times the
 // query heads of the group) and a run of key tiles. A warp owns a part of each tile (16 or 32 keys, 8 in fp32)
 // and has a ring of stages of its own, filled by 16-byte cp.async: page lookups run one tile ahead of the loads,
-// loads up to three tiles ahead of the products and on across item boundaries, and no warp waits for
+// loads one tile ahead of the products (two in fp32, except for 8 rows of 128) and on across item boundaries, and no warp waits for
 // another until an item's end. Rows that are not there (behind the last key, on a bad page) are
 // filled with zeros and masked, so whatever lies in unused rows of a page is never read.
-// 256 x 12 heads x 128..1000 keys x 64 fp16: 82 us, 5.2 TB/s (78 % of the copy rate); 32 x 10/2 heads x 300..2000 x 128 bf16: 20 us, of
+// 256 x 12 heads x 128..1000 keys x 64 fp16: 84 us, 5.1 TB/s (77 % of the copy rate); 32 x 10/2 heads x 300..2000 x 128 bf16: 20 us, of
 // which the keys and values need 6 (finding shares, first loads, joining and launches the rest).
 //   half: transposed products by mma.sync (m16n8k16), S^T = K Q^T and O^T += V^T P^T, so that the keys fill
 //         the 16 rows of an MMA and the queries are its 8 columns: with one to eight rows per item (decoding) half the products,
@@ -534,7 +534,8 @@ static int launch_few(const PagedAttnParams& p, cudaStream_t st) {
   if (int rc = limit.raise((const void*)kern, Cfg::kSmem)) return rc;
   const int grid = Cfg::kBlocks * sm_count();
   // Tables that end within a few tiles: no item is cut then, and there is nothing to join (a second launch costs 3 us, as
-  // much as six tiles one after the other).
+  // much as six tiles one after the other). The host knows the table's width and not the lengths: one request of 144 keys, 12 heads of
+  // 64 in fp32, takes 16 us with a table cut to its size and 22 with one of 2048 positions.
   const int whole = (int64_t)p.width * p.page.d <= 6 * Cfg::KT;
   TempBuf part(whole ? 0 : partial_bytes(grid, M, D), st, Scratch::kOwnPool);
   if (!part.ok()) return MT_ERR_CUDA;

@@ -25,7 +25,7 @@
 //
 // Roofline: tensor pipe, 4 D operations per (row, visible key), or the exponentials (16 per clock per SM,
 // 1024 cycles per 128x128 tile, the MMA's time at D = 128 and twice it at D = 64). 2 x 1024 new tokens over 8000..14000 keys, 10/2
-// heads of 128, bf16: 131 us, 890 TFLOP/s (a step of 128 keys takes 3400 cycles: a subtile's softmax, 2100, and its products behind
+// heads of 128, bf16: 138 us, 840 TFLOP/s (a step of 128 keys takes 3400 cycles: a subtile's softmax, 2100, and its products behind
 // it, 1340; ordering the subtiles' exponentials changes nothing, a quarter of them as polynomials costs 20 % in instructions).
 #include "attention_paged.cuh"
 #include "paged_work.cuh"
