@@ -79,8 +79,12 @@ class PagedKVCache:
             self.max_new, self.rows = int(counts.max()), n
             self._idle = np.flatnonzero(np.diff(np.r_[0, fresh == 0, 0])).reshape(-1, 2).tolist()     # [first, end) of requests without new tokens
             self._fresh = fresh.copy()
-        K.fused_paged_tables(self._held, self._fresh_dev, self.tables, self.free_pages, self._n_free, self.page_size,
-                             out=(self.starts, self._kv_len, self.position, self.slot, self._next_free))
+        try:
+            K.fused_paged_tables(self._held, self._fresh_dev, self.tables, self.free_pages, self._n_free, self.page_size,
+                                 out=(self.starts, self._kv_len, self.position, self.slot, self._next_free))
+        except Exception:
+            self._end()                                          # nothing was written there
+            raise
         self._held, self._kv_len = self._kv_len, self._held
         self._n_free, self._next_free = self._next_free, self._n_free
         self.lengths = after

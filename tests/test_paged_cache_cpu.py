@@ -298,3 +298,21 @@ def test_a_refused_generate_leaves_the_model_as_it_was():
     with pytest.raises(ValueError):
         GPT.generate(model, [[1, 2], []], 3)
     assert model.training
+
+
+def test_a_step_that_the_library_refused(paged, monkeypatch):
+    """Its positions and slots were never written: no forward can run it, and the cache is as before."""
+    def refuse(*a, **k):
+        raise RuntimeError("refused")
+    cache, other = step(a_cache(paged), [3, 5]), step(a_cache(paged), [3, 5])
+    for fresh in ([1, 1], [3, 5]):                               # with arrays made anew, and with those of the step before
+        with monkeypatch.context() as m:
+            m.setattr(paged.K, "fused_paged_tables", refuse)
+            with pytest.raises(RuntimeError):
+                cache.begin(fresh)
+        with pytest.raises(ValueError):
+            cache.check((1, sum(fresh)), 2, 1, 64, 16)
+        with pytest.raises(RuntimeError):
+            fill(cache)
+        same_state(cache, other)
+    same_state(step(cache, [1, 1]), step(other, [1, 1]))
