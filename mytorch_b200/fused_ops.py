@@ -459,9 +459,9 @@ def fused_paged_attention(q, k_pages, v_pages, tables, starts, kv_len, max_new=N
     """Attention of the new rows q [N, H, D], packed by `starts` [R+1], over the pages that `tables` [R, width]
     lists: kv_len [R] keys per request, this step's among them, causal (mt_attn_paged; grouped-query where H is
     a multiple of the pools' heads). -> o [N, H, D]; rows that no request has keep what `out` held (0 without
-    `out`). max_new: the most new rows of one request, where the caller knows it; it picks the kernel, and without it
-    the one for many rows is taken, slower for single tokens (32 requests, 10/2 heads: 31 us against 19) and with the
-    weights rounded to half precision.
+    `out`). max_new: the most new rows of one request, where the caller knows it; it picks the kernel. Without it all rows may
+    be one request's, and many (beyond 32 with H / Hkv, 8 in fp32) go to the kernel for many rows: slower for single tokens (32
+    requests, 10/2 heads: 31 us against 19) and, in half precision, with the weights rounded to the type.
     `strides` (Strides3, batch unused) reads q as a view. Not differentiable: a cache holds no graph."""
     q = _A(q)
     k_pages, v_pages = _pools(k_pages, v_pages)
